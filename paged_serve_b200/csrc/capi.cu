@@ -3,6 +3,7 @@
 // runtime, so the library does not link libcuda directly).
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "capi_internal.h"
@@ -43,9 +44,10 @@ int check_launch(const char* what) {
   return PS_OK;
 }
 
-int encode_tmap_16bit(CUtensorMap* map, void* base, int rank, const uint64_t* dims,
-                      const uint64_t* strides_bytes, const uint32_t* box,
-                      CUtensorMapSwizzle swizzle) {
+namespace {
+int encode_tmap(CUtensorMap* map, CUtensorMapDataType type, void* base, int rank,
+                const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
+                CUtensorMapSwizzle swizzle) {
   std::call_once(g_encode_once, load_encode);
   if (g_encode == nullptr) {
     return fail(PS_ERR_CUDA, "cuTensorMapEncodeTiled unavailable (%s)",
@@ -61,8 +63,7 @@ int encode_tmap_16bit(CUtensorMap* map, void* base, int rank, const uint64_t* di
     estride[i] = 1;
     if (i > 0) gstride[i - 1] = strides_bytes[i - 1];
   }
-  CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, base, gdim, gstride, bdim,
-                        estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+  CUresult r = g_encode(map, type, rank, base, gdim, gstride, bdim, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return fail(PS_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
@@ -70,11 +71,11 @@ int encode_tmap_16bit(CUtensorMap* map, void* base, int rank, const uint64_t* di
   return PS_OK;
 }
 
-namespace {
 struct TmapCacheEntry {
   const void* base = nullptr;
   uint64_t rows = 0;
   int d = 0;
+  int elem_bytes = 0;
   int box_rows = 0;
   CUtensorMap map;
 };
@@ -82,25 +83,40 @@ thread_local TmapCacheEntry g_tmap_cache[128];
 thread_local int g_tmap_next = 0;
 }  // namespace
 
-int get_pool_tmap(const void* pool, uint64_t rows, int head_dim, int box_rows, CUtensorMap* out) {
+int encode_tmap_16bit(CUtensorMap* map, void* base, int rank, const uint64_t* dims,
+                      const uint64_t* strides_bytes, const uint32_t* box,
+                      CUtensorMapSwizzle swizzle) {
+  return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, rank, dims, strides_bytes, box,
+                     swizzle);
+}
+
+int get_pool_tmap(const void* pool, uint64_t rows, int head_dim, int box_rows, CUtensorMap* out,
+                  int elem_bytes) {
   for (auto& e : g_tmap_cache) {
-    if (e.base == pool && e.rows == rows && e.d == head_dim && e.box_rows == box_rows) {
+    if (e.base == pool && e.rows == rows && e.d == head_dim && e.box_rows == box_rows &&
+        e.elem_bytes == elem_bytes) {
       *out = e.map;
       return PS_OK;
     }
   }
   const uint64_t dims[2] = {static_cast<uint64_t>(head_dim), rows};
-  const uint64_t strides[1] = {static_cast<uint64_t>(head_dim) * 2};
-  const uint32_t box[2] = {64, static_cast<uint32_t>(box_rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(head_dim) * elem_bytes};
+  const uint32_t cols = std::min(head_dim, 128 / elem_bytes);
+  const uint32_t box[2] = {cols, static_cast<uint32_t>(box_rows)};
   CUtensorMap map;
-  int st = encode_tmap_16bit(&map, const_cast<void*>(pool), 2, dims, strides, box,
-                             CU_TENSOR_MAP_SWIZZLE_128B);
+  int st = encode_tmap(&map,
+                       elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                       : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                       const_cast<void*>(pool), 2, dims, strides, box,
+                       cols * elem_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                               : CU_TENSOR_MAP_SWIZZLE_128B);
   if (st != PS_OK) return st;
   TmapCacheEntry& e = g_tmap_cache[g_tmap_next];
   g_tmap_next = (g_tmap_next + 1) % 128;
   e.base = pool;
   e.rows = rows;
   e.d = head_dim;
+  e.elem_bytes = elem_bytes;
   e.box_rows = box_rows;
   e.map = map;
   *out = map;

@@ -21,74 +21,10 @@
 // enough TMA bytes in flight per SM (NW * NS * 2 tiles per CTA).
 #include <cudaTypedefs.h>
 
-#include <algorithm>
-#include <mutex>
-#include <type_traits>
-
-#include "capi_internal.h"
-#include "common.cuh"
+#include "decode_common.cuh"
 
 namespace ps {
 namespace {
-
-constexpr int kChunk = 16;  // keys per MMA step (one 16-row TMA tile per K and V half)
-
-struct DecodeParams {
-  void* out;
-  const void* q;
-  int64_t out_stride;
-  int64_t q_stride;
-  const int32_t* block_tables;
-  int64_t bt_stride;
-  const int32_t* ctx_lens;
-  float* ws_o;    // [B][max_splits][Hq][D]
-  float* ws_lse;  // [B][max_splits][Hq]   (log2 domain)
-  int64_t num_blocks;
-  int num_seqs;
-  int num_launch;  // launch positions: num_seqs, or the length of a listed subset
-  int num_q_heads;
-  int num_kv_heads;
-  int group;  // Hq / Hkv
-  int max_blocks;
-  int block_size;
-  int part_tokens;  // partition length (multiple of 16 and of the block size)
-  int max_splits;
-  int table_cap;  // ints of block table staged per CTA
-  float scale_log2;
-  int32_t* err;
-  // Split-K only: the (sequence, partition) pairs that have keys, as
-  // b * max_splits + split, and their number; written by decode_plan_kernel.
-  int32_t* items;
-  int32_t* item_count;
-  int32_t* item_next;  // claim counter of the persistent CTAs (reset by the plan and the combine)
-  bool planned;        // the unit list was written by ps_paged_decode_plan for this step
-  // Optional permutation of [0, num_seqs) (longest first, from
-  // ps_paged_decode_order): the order CTAs / planned units take sequences in.
-  const int32_t* seq_order;
-  // Optional fused append of the step's new token (ps_paged_decode_append):
-  // new_k/new_v [num_seqs][Hkv][D] rows go to slot new_slots[b] of the pools
-  // (raw pointers; -1 = no token) before the unit that reads that slot loads it.
-  void* k_pool_w;
-  void* v_pool_w;
-  const void* new_k;
-  const void* new_v;
-  int64_t new_k_stride;
-  int64_t new_v_stride;
-  const int64_t* new_slots;
-  int64_t num_slots;
-};
-
-// Sequence at position i of the launch order; -1 (and an error bit) for an
-// entry that is not a sequence index.
-__device__ __forceinline__ int ordered_seq(const DecodeParams& p, int i) {
-  if (!p.seq_order) return i;
-  const int b = p.seq_order[i];
-  if (b < 0 || b >= p.num_seqs) {
-    set_device_error(p.err, PS_DEVERR_LENGTH);
-    return -1;
-  }
-  return b;
-}
 
 template <int D>
 struct TileGeom {
@@ -565,139 +501,6 @@ __global__ void __launch_bounds__(1024) decode_order_kernel(const int32_t* ctx_l
   for (int b = t; b < n; b += 1024) order[atomicAdd(&cursor[bucket(ctx_lens[b])], 1)] = b;
 }
 
-// Lists the (sequence, partition) units of a split-K launch in launch order
-// (seq_order when given, else batch order):
-// a sequence with ctx keys has ceil(ctx / part) partitions, and one unit even
-// without keys (its output is written as zeros). One CTA of 1024 threads; a
-// running block-wide prefix sum places each sequence's units.
-__global__ void __launch_bounds__(1024) decode_plan_kernel(const DecodeParams p) {
-  pdl_trigger();
-  pdl_wait();
-  __shared__ int wsum[32];
-  __shared__ int carry;
-  const int lane = threadIdx.x & 31;
-  const int warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) carry = 0;
-  __syncthreads();
-  for (int base = 0; base < p.num_launch; base += 1024) {
-    const int i = base + threadIdx.x;
-    const int b = i < p.num_launch ? ordered_seq(p, i) : -1;
-    int ns = 0;
-    if (b >= 0) {
-      int ctx = p.ctx_lens[b];
-      if (ctx > p.max_blocks * p.block_size) ctx = 0;  // the decode kernel reports it
-      ns = ctx <= 0 ? 1 : (ctx + p.part_tokens - 1) / p.part_tokens;
-    }
-    int x = ns;  // inclusive scan within the warp
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) wsum[warp] = x;
-    __syncthreads();
-    if (warp == 0) {
-      const int w = wsum[lane];
-      int y = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int z = __shfl_up_sync(0xffffffffu, y, o);
-        if (lane >= o) y += z;
-      }
-      wsum[lane] = y - w;  // exclusive, per warp
-    }
-    __syncthreads();
-    const int off = carry + wsum[warp] + x - ns;
-    for (int k = 0; k < ns; ++k) p.items[off + k] = b * p.max_splits + k;
-    __syncthreads();  // every thread has read carry
-    if (threadIdx.x == blockDim.x - 1) carry = off + ns;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    *p.item_count = carry;
-    *p.item_next = 0;
-  }
-}
-
-// Merge the partitions of each split sequence: out = sum_s w_s O_s, with
-// w_s = 2^(lse_s - max lse) / sum. One warp per (sequence, query head).
-template <typename T, int D>
-__global__ void __launch_bounds__(128) decode_combine_kernel(const DecodeParams p) {
-  pdl_trigger();
-  pdl_wait();
-  // The decode launch has finished claiming units: rearm the claim counter, so
-  // the next layer of a planned step can reuse the unit list without a plan.
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.item_next = 0;
-  const int warp_global = blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (warp_global >= p.num_launch * p.num_q_heads) return;
-  const int b = ordered_seq(p, warp_global / p.num_q_heads);  // only launched sequences
-  if (b < 0) return;
-  const int qh = warp_global % p.num_q_heads;
-  int ctx = p.ctx_lens[b];
-  if (ctx > p.max_blocks * p.block_size) ctx = 0;
-  const int nsplit = (ctx + p.part_tokens - 1) / p.part_tokens;
-  if (nsplit <= 1) return;
-  const int64_t base = static_cast<int64_t>(b) * p.max_splits * p.num_q_heads + qh;
-  float mmax = -INFINITY;
-  for (int s = lane; s < nsplit; s += 32)
-    mmax = fmaxf(mmax, p.ws_lse[base + static_cast<int64_t>(s) * p.num_q_heads]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mmax = fmaxf(mmax, __shfl_xor_sync(0xffffffffu, mmax, o));
-  constexpr int kPer = D / 32;  // dims per lane
-  using Vec = typename std::conditional<kPer == 4, float4, float2>::type;
-  float acc[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-  float wsum = 0.f;
-  auto add = [&](float w, const Vec& v) {
-    wsum += w;
-    acc[0] += w * v.x;
-    acc[1] += w * v.y;
-    if constexpr (kPer == 4) {
-      acc[2] += w * reinterpret_cast<const float4&>(v).z;
-      acc[3] += w * reinterpret_cast<const float4&>(v).w;
-    }
-  };
-  auto load = [&](int s) {
-    return *reinterpret_cast<const Vec*>(p.ws_o + (base + static_cast<int64_t>(s) * p.num_q_heads) * D +
-                                         lane * kPer);
-  };
-  // Partitions in order (the sum order is fixed); lane l computes the weight of
-  // partition s0 + l. Eight partitions' loads are in flight at a time: when few
-  // sequences are split, the longest one's chain of loads (64 partitions for
-  // 32k tokens) sets the length of the launch (four in flight: 156.6 against
-  // 153.3 us per 64-sequence 70B layer); sixteen gain a little more there but
-  // cost occupancy when many sequences are split.
-  for (int s0 = 0; s0 < nsplit; s0 += 32) {
-    const int n = min(32, nsplit - s0);
-    const float lse = lane < n ? p.ws_lse[base + static_cast<int64_t>(s0 + lane) * p.num_q_heads]
-                               : -INFINITY;
-    const float wl = (lse == -INFINITY) ? 0.f : exp2f(lse - mmax);
-    int k = 0;
-    for (; k + 8 <= n; k += 8) {
-      Vec v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = load(s0 + k + u);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) add(__shfl_sync(0xffffffffu, wl, k + u), v[u]);
-    }
-    for (; k + 4 <= n; k += 4) {
-      Vec v[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = load(s0 + k + u);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) add(__shfl_sync(0xffffffffu, wl, k + u), v[u]);
-    }
-    for (; k < n; ++k) add(__shfl_sync(0xffffffffu, wl, k), load(s0 + k));
-  }
-  const float inv = (wsum > 0.f) ? 1.f / wsum : 0.f;
-  T* orow = static_cast<T*>(p.out) + b * p.out_stride + static_cast<int64_t>(qh) * D + lane * kPer;
-#pragma unroll
-  for (int i = 0; i < kPer; i += 2)
-    *reinterpret_cast<uint32_t*>(orow + i) = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
-}
-
 // ------------------------------------------------------------ host side
 constexpr int kNW = 4;  // warps per CTA
 constexpr int kNS = 2;  // TMA stages per warp
@@ -710,31 +513,6 @@ constexpr int kNS = 2;  // TMA stages per warp
 // (eight: 381 against 347 us per 8B layer).
 template <int D>
 constexpr int unsplit_warps() { return D == 64 ? 8 : kNW; }
-
-int effective_part_tokens(int split_tokens, int max_blocks, int block_size) {
-  return split_tokens > 0 ? split_tokens : max_blocks * block_size;
-}
-
-// Guards the per-device launch caches below against concurrent host threads.
-std::mutex g_launch_mu;
-
-// The dynamic shared-memory attribute is per function and per device; raise it
-// only when a larger block table than any seen so far needs more.
-template <typename K>
-int reserve_smem(K kern, size_t smem, size_t (&configured)[64]) {
-  std::lock_guard<std::mutex> lock(g_launch_mu);
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || configured[dev] < smem) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(smem));
-    if (e != cudaSuccess)
-      return fail(PS_ERR_CUDA, "ps_paged_decode: cannot reserve %zu B shared memory: %s", smem,
-                  cudaGetErrorString(e));
-    if (dev >= 0 && dev < 64) configured[dev] = smem;
-  }
-  return PS_OK;
-}
 
 template <typename T, int D, int BS, int R>
 int launch_decode(const DecodeParams& p, const CUtensorMap& km, const CUtensorMap& vm,
@@ -879,64 +657,6 @@ struct NewToken {
   const int64_t* slots;
 };
 
-// Argument checks shared by every decode entry point; on success fills the
-// partition length (tokens), the partitions per sequence and the block-table
-// window a partition spans. Returns PS_OK, or the status of the first failure
-// with its message naming `fn`.
-int validate_decode(const char* fn, const void* out, int64_t out_seq_stride, const void* query,
-                    int64_t query_seq_stride, const void* k_pool, const void* v_pool,
-                    int64_t num_blocks, const int32_t* block_tables, int64_t block_table_stride,
-                    const int32_t* ctx_lens, int num_seqs, int num_q_heads, int num_kv_heads,
-                    int head_dim, int block_size, int max_blocks_per_seq, int split_tokens,
-                    int dtype, int* part_out, int* max_splits_out, int* table_cap_out) {
-  if (dtype != PS_DTYPE_BF16 && dtype != PS_DTYPE_F16)
-    return fail(PS_ERR_UNSUPPORTED, "%s: dtype %d unsupported (bf16/f16 only)", fn, dtype);
-  if (head_dim != 64 && head_dim != 128)
-    return fail(PS_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (64 or 128)", fn, head_dim);
-  if (block_size != 8 && block_size != 16 && block_size != 32)
-    return fail(PS_ERR_UNSUPPORTED, "%s: block_size %d unsupported (8, 16 or 32)", fn,
-                block_size);
-  if (num_seqs < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_blocks <= 0 ||
-      max_blocks_per_seq <= 0)
-    return fail(PS_ERR_INVALID, "%s: bad sizes", fn);
-  if (num_q_heads % num_kv_heads != 0)
-    return fail(PS_ERR_INVALID, "%s: num_q_heads %d not divisible by num_kv_heads %d", fn,
-                num_q_heads, num_kv_heads);
-  const int group = num_q_heads / num_kv_heads;
-  if (group > 16)
-    return fail(PS_ERR_UNSUPPORTED, "%s: %d query heads per kv head unsupported (max 16)", fn, group);
-  if (num_seqs == 0) return PS_OK;  // nothing to launch; the caller checks num_seqs too
-  if (num_seqs > 65535 || num_kv_heads > 65535)
-    return fail(PS_ERR_INVALID, "%s: too many sequences/heads for one launch", fn);
-  if (!out || !query || !k_pool || !v_pool || !block_tables || !ctx_lens)
-    return fail(PS_ERR_INVALID, "%s: null pointer argument", fn);
-  if (block_table_stride < max_blocks_per_seq)
-    return fail(PS_ERR_INVALID, "%s: block_table_stride < max_blocks_per_seq", fn);
-  if (query_seq_stride < static_cast<int64_t>(num_q_heads) * head_dim ||
-      out_seq_stride < static_cast<int64_t>(num_q_heads) * head_dim || (query_seq_stride % 8) ||
-      (out_seq_stride % 8) || !aligned(query, 16) || !aligned(out, 16))
-    return fail(PS_ERR_INVALID, "%s: query/out must be 16-byte aligned, strides >= Hq*D and %% 8", fn);
-  if (!aligned(k_pool, 16) || !aligned(v_pool, 16))
-    return fail(PS_ERR_INVALID, "%s: pools must be 16-byte aligned", fn);
-  const int64_t rows = num_blocks * num_kv_heads * block_size;
-  if (rows >= (int64_t(1) << 31))
-    return fail(PS_ERR_INVALID, "%s: pool too large for 32-bit TMA row coordinates", fn);
-  const int unit = block_size > kChunk ? block_size : kChunk;
-  if (split_tokens < 0 || (split_tokens % unit))
-    return fail(PS_ERR_INVALID, "%s: split_tokens must be >= 0 and a multiple of %d", fn, unit);
-  const int part = effective_part_tokens(split_tokens, max_blocks_per_seq, block_size);
-  const int max_splits = (max_blocks_per_seq * block_size + part - 1) / part;
-  const int table_cap = (part + block_size - 1) / block_size;
-  if (table_cap > 8192)
-    return fail(PS_ERR_UNSUPPORTED, "%s: partition of %d blocks too long; set split_tokens", fn,
-                table_cap);
-  if (max_splits > 65535) return fail(PS_ERR_INVALID, "%s: too many partitions", fn);
-  *part_out = part;
-  *max_splits_out = max_splits;
-  *table_cap_out = table_cap;
-  return PS_OK;
-}
-
 int decode_entry(const char* fn, void* out, int64_t out_seq_stride, const void* query,
                  int64_t query_seq_stride, const void* k_pool, const void* v_pool,
                  int64_t num_blocks, const int32_t* block_tables, int64_t block_table_stride,
@@ -958,23 +678,10 @@ int decode_entry(const char* fn, void* out, int64_t out_seq_stride, const void* 
 
   DecodeParams p{};
   if (max_splits > 1) {
-    const int64_t need = ps_paged_decode_workspace_bytes(num_seqs, num_q_heads, head_dim, block_size,
-                                                         max_blocks_per_seq, split_tokens);
-    if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
-      return fail(PS_ERR_INVALID, "%s: split-K needs a 256-byte aligned workspace of %lld bytes",
-                  fn, (long long)need);
-    if (static_cast<int64_t>(num_seqs) * max_splits >= (int64_t(1) << 31))
-      return fail(PS_ERR_INVALID, "%s: too many (sequence, partition) units", fn);
-    const int64_t rows_ws = static_cast<int64_t>(num_seqs) * max_splits * num_q_heads;
-    const int64_t o_bytes = ((rows_ws * head_dim * 4) + 255) / 256 * 256;
-    const int64_t lse_bytes = ((rows_ws * 4) + 255) / 256 * 256;
-    const int64_t item_bytes = ((static_cast<int64_t>(num_seqs) * max_splits * 4) + 255) / 256 * 256;
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
-    p.ws_o = reinterpret_cast<float*>(ws);
-    p.ws_lse = reinterpret_cast<float*>(ws + o_bytes);
-    p.items = reinterpret_cast<int32_t*>(ws + o_bytes + lse_bytes);
-    p.item_count = reinterpret_cast<int32_t*>(ws + o_bytes + lse_bytes + item_bytes);
-    p.item_next = p.item_count + 1;
+    const int st = set_split_workspace(fn, &p, num_seqs, num_q_heads, head_dim, block_size,
+                                       max_blocks_per_seq, split_tokens, max_splits, workspace,
+                                       workspace_bytes);
+    if (st != PS_OK) return st;
   }
   p.out = out;
   p.q = query;
