@@ -57,6 +57,10 @@ extern "C" {
 #define PS_DTYPE_F16 1
 #define PS_DTYPE_BF16 2
 
+/* ---- code types of an 8-bit KV cache (ps_cache_append_quant and the entry points beside it) ---- */
+#define PS_CODE_E4M3 1
+#define PS_CODE_INT8 2
+
 /* ---- device error bits ORed into *device_error ---- */
 #define PS_DEVERR_BLOCK_ID 1   /* block table entry outside [0, num_blocks)            */
 #define PS_DEVERR_SLOT 2       /* slot_mapping entry outside [-1, num_blocks*block_size) */
@@ -462,6 +466,99 @@ PS_API int ps_paged_prefill_split(void* out, int64_t out_token_stride, const voi
 PS_API int64_t ps_paged_prefill_workspace_bytes(int num_seqs, int max_q_len, int num_q_heads,
                                                 int num_kv_heads, int head_dim, int block_size,
                                                 int max_blocks_per_seq, int split_keys);
+
+/*
+ * ---- 8-bit KV cache ----
+ *
+ * The pools hold one code per value, in the layout of the 16-bit pools
+ * (pool[num_blocks][num_kv_heads][block_size][head_dim], one byte each), and a
+ * scale pool of float32 [num_blocks][num_kv_heads][block_size] beside each: the
+ * value is code * scale. No counterpart exists in the reference, whose cache
+ * holds the model's dtype. For a row x (one token of one KV head):
+ *     scale = max(max|x| / qmax, 2^-126),  qmax = 448 (PS_CODE_E4M3) or 127 (PS_CODE_INT8)
+ *     code  = round(x * (1 / scale)), ties to even
+ * every operation rounded to float32, so the codes are reproducible to the bit.
+ * A row with a NaN or an infinity gets a NaN scale: all its values read back as NaN. Blocks move with ps_copy_blocks / ps_swap_blocks: codes with
+ * block_bytes = num_kv_heads*block_size*head_dim, scales (called the same way with the
+ * scale pools) with num_kv_heads*block_size*4.
+ */
+
+/*
+ * ps_cache_append_quant — ps_cache_append into an 8-bit cache.
+ *
+ * key/value/slot_mapping and strides as in ps_cache_append; dtype is the type of
+ * key and value, code the pools' code type. Pools, scales, key and value must be
+ * 16-byte aligned.
+ */
+PS_API int ps_cache_append_quant(void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                                 const void* key, const void* value, const int64_t* slot_mapping,
+                                 int64_t num_tokens, int64_t key_token_stride,
+                                 int64_t value_token_stride, int num_kv_heads, int head_dim,
+                                 int block_size, int64_t num_blocks, int dtype, int code,
+                                 int32_t* device_error, void* stream);
+
+/*
+ * ps_cache_append_rope_quant — ps_cache_append_quant with split-half RoPE on K.
+ *
+ * positions and cos_sin_table as in ps_cache_append_rope. K is rotated in float32
+ * and quantised from there: products of two 16-bit values are exact in float32, so
+ * the rotated value is rounded once (ps_cache_append_rope, which reproduces the
+ * reference's arithmetic, rounds to the storage type three times).
+ */
+PS_API int ps_cache_append_rope_quant(void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                                      const void* key, const void* value,
+                                      const int64_t* slot_mapping, const int64_t* positions,
+                                      int64_t num_tokens, int64_t key_token_stride,
+                                      int64_t value_token_stride, int num_kv_heads, int head_dim,
+                                      int block_size, int64_t num_blocks,
+                                      const void* cos_sin_table, int64_t table_positions,
+                                      int rope_dim, int dtype, int code, int32_t* device_error,
+                                      void* stream);
+
+/*
+ * ps_cache_read_quant — an 8-bit cache's tokens back as 16-bit values.
+ *
+ * Block j of sequence b (j < ceil(ctx_lens[b] / block_size)) is read from pool block
+ * block_tables[b][j] and written as code * scale, rounded once to dtype, to block
+ * out_tables[b][j] of k_out/v_out ([num_out_blocks][num_kv_heads][block_size][head_dim]).
+ * Rows past the last token are written as zeros; other blocks of the output are
+ * left as they are. ps_paged_prefill and ps_paged_decode_shared then run on
+ * k_out/v_out with out_tables. Output blocks that two sequences name are written
+ * twice (concurrently: name them twice only for the same source block, whole in both).
+ * Ids outside their pool set PS_DEVERR_BLOCK_ID and the block is skipped; a length
+ * beyond max_blocks_per_seq blocks sets PS_DEVERR_LENGTH and the sequence is skipped.
+ */
+PS_API int ps_cache_read_quant(const void* k_pool, const void* v_pool, const float* k_scale,
+                               const float* v_scale, int64_t num_blocks, void* k_out, void* v_out,
+                               int64_t num_out_blocks, const int32_t* block_tables,
+                               int64_t block_table_stride, const int32_t* out_tables,
+                               int64_t out_table_stride, const int32_t* ctx_lens, int num_seqs,
+                               int num_kv_heads, int head_dim, int block_size,
+                               int max_blocks_per_seq, int dtype, int code, int32_t* device_error,
+                               void* stream);
+
+/*
+ * ps_paged_decode_quant — ps_paged_decode over an 8-bit cache.
+ *
+ * Arguments as ps_paged_decode (geometry, split_tokens, workspace, errors), with the
+ * scale pools, and: seq_list = launch order or subset as in ps_paged_decode_ordered /
+ * ps_paged_decode_listed (may be NULL with num_listed < 0); num_listed < 0 = all
+ * num_seqs sequences, else the entries of seq_list to run; planned != 0 = the unit
+ * list for these lengths, order and geometry is already in the workspace
+ * (ps_paged_decode_plan), all sequences. Keys at or past ctx_lens[b] are not
+ * used, whatever their rows and scales hold. Scores, softmax and accumulation are
+ * float32; probabilities times V scales are rounded to fp16 for the second product.
+ */
+PS_API int ps_paged_decode_quant(void* out, int64_t out_seq_stride, const void* query,
+                                 int64_t query_seq_stride, const void* k_pool, const void* v_pool,
+                                 const float* k_scale, const float* v_scale, int64_t num_blocks,
+                                 const int32_t* block_tables, int64_t block_table_stride,
+                                 const int32_t* ctx_lens, int num_seqs, const int32_t* seq_list,
+                                 int num_listed, int num_q_heads, int num_kv_heads, int head_dim,
+                                 int block_size, int max_blocks_per_seq, float scale,
+                                 int split_tokens, int planned, void* workspace,
+                                 int64_t workspace_bytes, int dtype, int code,
+                                 int32_t* device_error, void* stream);
 
 /*
  * ps_stream_read — diagnostic: read num_bytes of device memory once and XOR every

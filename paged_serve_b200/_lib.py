@@ -23,6 +23,9 @@ PS_ERR_CUDA = 3
 PS_DTYPE_F16 = 1
 PS_DTYPE_BF16 = 2
 
+PS_CODE_E4M3 = 1
+PS_CODE_INT8 = 2
+
 PS_DEVERR_BLOCK_ID = 1
 PS_DEVERR_SLOT = 2
 PS_DEVERR_POSITION = 4
@@ -84,6 +87,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [_p, _l, _p, _l, _p, _p, _l, _p, _l, _p, _i, _i, _i, _i, _i, _i, c_float, _i, _i, _p,
          _p],
+    ),
+    "ps_cache_append_quant": (
+        c_int, [_p, _p, _p, _p, _p, _p, _p, _l, _l, _l, _i, _i, _i, _l, _i, _i, _p, _p],
+    ),
+    "ps_cache_append_rope_quant": (
+        c_int,
+        [_p, _p, _p, _p, _p, _p, _p, _p, _l, _l, _l, _i, _i, _i, _l, _p, _l, _i, _i, _i, _p, _p],
+    ),
+    "ps_cache_read_quant": (
+        c_int,
+        [_p, _p, _p, _p, _l, _p, _p, _l, _p, _l, _p, _l, _p, _i, _i, _i, _i, _i, _i, _i, _p, _p],
+    ),
+    "ps_paged_decode_quant": (
+        c_int,
+        [_p, _l, _p, _l, _p, _p, _p, _p, _l, _p, _l, _p, _i, _p, _i, _i, _i, _i, _i, _i, c_float,
+         _i, _i, _p, _l, _i, _i, _p, _p],
     ),
     "ps_stream_read": (c_int, [_p, _l, _p, _i, _p, _p]),
     "ps_paged_prefill": (

@@ -1,0 +1,629 @@
+// Paged decode attention (one query token per sequence, GQA) over an 8-bit KV
+// cache (quant.cuh) for sm_100a.
+//
+// With codes k, v and per-row scales a_n (K) and b_n (V) of key n:
+//   s_n = scale * a_n * (q . k_n)     o = sum_n softmax(s)_n * b_n * v_n
+// so both scales stay outside the matrix products: a_n multiplies a score, b_n a
+// probability. The products run on fp16 warp MMAs: every e4m3 or int8 code is an
+// fp16 value, so only the probabilities are rounded (2^-12 relative); the
+// queries are first brought to [-2, 2) per head by a power of two (exact, up to
+// values below 2^-24 of the head's largest).
+//
+// A probability times b_n must fit fp16 too, whatever the b_n are, and keep its
+// precision where the sum has its weight. So beside the running maximum m of the
+// scores (for the softmax sum) each head has a running maximum M of
+// s_n + log2 b_n, and the second product takes
+//   P'_n = 2^(s_n + log2 b_n - M + 7)
+// Both maxima move only when passed by 8 (2^8), so P' is below 2^15.2 and a term
+// keeps fp16's full precision down to 2^-21 of the largest one; O is rescaled, in
+// fp32, when M moves.
+//
+// Work decomposition as in paged_decode.cu: one CTA per (KV head, sequence), or
+// persistent CTAs claiming (KV head, partition) units; each warp owns a ring of
+// stages of 32 keys filled by TMA (codes) and bulk copies (scales). The group of
+// query heads is the N side of the MMAs and the keys (for S) or the dims (for O)
+// the M side, so eight heads fill a tile that would be half padding the other
+// way round:
+//   S^T[16 keys x 8 heads] = K[16 x D] . Q^T      (D/16 MMAs)
+//   O^T[16 dims x 8 heads] += V^T[16 x 16 keys] . P^T
+// The K codes of four neighbouring dims reach a lane as one 32-bit register; which
+// of the MMA's k indices they stand for is free as long as Q is laid out alike.
+#include <cudaTypedefs.h>
+
+#include "decode_common.cuh"
+#include "quant.cuh"
+
+namespace ps {
+namespace {
+
+constexpr int kKeys = 32;  // keys per stage
+
+struct QuantDecodeParams {
+  DecodeParams d;
+  const float* k_scale;  // [num_blocks][Hkv][block_size]
+  const float* v_scale;
+};
+
+template <int D, int NW, int NS>
+struct QuantSmem {
+  static constexpr int kTileBytes = kKeys * D;  // K or V codes of one stage
+  static constexpr int kRingBytes = NW * NS * 2 * kTileBytes;
+  static constexpr int kScaleOffset = kRingBytes;  // per stage: 32 K scales, 32 V scales
+  static constexpr int kStageTx = 2 * kTileBytes + 2 * kKeys * 4;
+  static constexpr int kBarOffset = kScaleOffset + NW * NS * 2 * kKeys * 4;
+  static constexpr int kTableOffset = kBarOffset + NW * NS * 8;
+  static_assert(NW * 16 * (D + 2) * 4 <= kRingBytes, "merge area must fit in the ring");
+  static size_t bytes(int table_cap) {
+    return 1024 /*alignment slack*/ + kTableOffset + static_cast<size_t>(table_cap) * 4;
+  }
+  // Byte offset of 16-byte chunk c of key t inside a swizzled tile: a row of 128
+  // bytes spreads over 8 rows (128-byte swizzle), one of 64 bytes over 4 pairs of
+  // rows (64-byte swizzle); ldmatrix's 8 rows then hit 8 different banks groups.
+  __device__ __forceinline__ static uint32_t off(int t, int c) {
+    return D == 128 ? t * 128 + ((c ^ (t & 7)) << 4) : t * 64 + ((c ^ ((t >> 1) & 3)) << 4);
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Transposes an 8x8 matrix of 16-bit elements held two per lane.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// T = type of the queries and the output; C = code type; R = 8 or 16 head
+// columns; kList as in paged_decode_kernel.
+template <typename T, typename C, int D, int NW, int NS, int BS, int R, bool kList>
+__global__ void __launch_bounds__(NW * 32)
+    paged_decode_quant_kernel(const QuantDecodeParams qp, const __grid_constant__ CUtensorMap kmap,
+                              const __grid_constant__ CUtensorMap vmap) {
+  static_assert(R == 8 || R == 16, "8 or 16 head columns");
+  using SM = QuantSmem<D, NW, NS>;
+  const DecodeParams& p = qp.d;
+  constexpr int kNT = R / 8;       // head tiles
+  constexpr int kKSteps = D / 16;  // k steps of S, dim tiles of O
+  constexpr int kBox = BS < kKeys ? BS : kKeys;
+  constexpr int kBoxes = kKeys / kBox;
+
+  int h = blockIdx.x;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int group = p.group;
+  const int r = lane >> 2;  // key (S) or dim pair (O) row
+  const int q4 = lane & 3;  // heads 2 q4, 2 q4 + 1 of a head tile
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::kBarOffset);
+  int32_t* table = reinterpret_cast<int32_t*>(smem + SM::kTableOffset);
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
+    for (int i = 0; i < NW * NS; ++i) mbar_init(&bars[i], 1);
+    fence_barrier_init();
+  }
+  pdl_wait();
+
+  __shared__ int claimed[2];
+  int total = 0, next = 0;
+  if constexpr (kList) {
+    const int cap = p.num_seqs * p.max_splits;
+    total = min(max(*p.item_count, 0), cap) * p.num_kv_heads;
+    if (threadIdx.x == 0) next = atomicAdd(p.item_next, 1);
+  }
+  uint32_t gbase = 0;  // this warp's ring iterations so far
+  for (int k = 0;; ++k) {
+    int split, b;
+    if constexpr (kList) {
+      if (threadIdx.x == 0) {
+        claimed[k & 1] = next;
+        next = atomicAdd(p.item_next, 1);
+      }
+      __syncthreads();
+      const int u = claimed[k & 1];
+      if (u >= total) break;
+      h = u % p.num_kv_heads;
+      const int item = p.items[u / p.num_kv_heads];
+      if (item < 0 || item >= p.num_seqs * p.max_splits) {
+        if (threadIdx.x == 0) set_device_error(p.err, PS_DEVERR_LENGTH);
+        continue;
+      }
+      split = item % p.max_splits;
+      b = item / p.max_splits;
+    } else {
+      if (k > 0) break;
+      split = 0;
+      b = ordered_seq(p, blockIdx.z);
+      if (b < 0) break;
+    }
+
+    int ctx = p.ctx_lens[b];
+    if (ctx > p.max_blocks * BS) {
+      if (threadIdx.x == 0 && split == 0) set_device_error(p.err, PS_DEVERR_LENGTH);
+      ctx = 0;
+    }
+    const int nsplit = (ctx + p.part_tokens - 1) / p.part_tokens;
+    if (ctx <= 0) {
+      if (split == 0) {
+        T* o = static_cast<T*>(p.out) + b * p.out_stride + static_cast<int64_t>(h) * group * D;
+        for (int i = threadIdx.x; i < group * D; i += blockDim.x) o[i] = from_f32<T>(0.f);
+      }
+      continue;
+    }
+    if (split >= nsplit) continue;
+
+    const int t_begin = split * p.part_tokens;
+    const int n_keys = min(ctx - t_begin, p.part_tokens);
+    const int nchunk = (n_keys + kKeys - 1) / kKeys;
+    const int nblk = (n_keys + BS - 1) / BS;
+    const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride + t_begin / BS;
+    for (int i = threadIdx.x; i < nblk; i += blockDim.x) {
+      int32_t id = bt[i];
+      if (id < 0 || id >= p.num_blocks) {
+        set_device_error(p.err, PS_DEVERR_BLOCK_ID);
+        id = 0;  // read a valid block instead of faulting; the error bit reports it
+      }
+      table[i] = id;
+    }
+    __syncthreads();
+
+    // Loads of warp-local iteration `it` (keys [32 j, 32 j + 32), j = warp + it NW):
+    // lane x of the first 4 kBoxes issues one copy (K codes, V codes, K scales,
+    // V scales of one box).
+    auto issue = [&](int it) {
+      const int j = warp + it * NW;
+      const int st = warp * NS + (gbase + it) % NS;
+      if (lane == 0) mbar_arrive_expect_tx(&bars[st], SM::kStageTx);
+      __syncwarp();
+      if (lane < 4 * kBoxes) {
+        const int x = lane >> 2;
+        const int what = lane & 3;
+        const int tok = j * kKeys + x * kBox;
+        // A box past the partition's last block re-reads that block (its keys are masked).
+        const int bi = min(tok / BS, nblk - 1);
+        const int64_t row = (static_cast<int64_t>(table[bi]) * p.num_kv_heads + h) * BS + tok % BS;
+        if (what < 2) {
+          tma_load_2d(smem + (st * 2 + what) * SM::kTileBytes + x * kBox * D, what ? &vmap : &kmap,
+                      &bars[st], 0, static_cast<int32_t>(row));
+        } else {
+          bulk_g2s(smem + SM::kScaleOffset + (st * 2 + what - 2) * kKeys * 4 + x * kBox * 4,
+                   (what == 2 ? qp.k_scale : qp.v_scale) + row, kBox * 4, &bars[st]);
+        }
+      }
+    };
+#pragma unroll
+    for (int it = 0; it < NS; ++it)
+      if (warp + it * NW < nchunk) issue(it);
+
+    // Q as the B operand: lane holds head n = lane/4 of each head tile, dims
+    // 16 kk + 4 q4 .. + 3 of k step kk, as fp16 times 2^-e_head. The factor that
+    // turns an S element of heads 2 q4, 2 q4 + 1 into log2 units goes to qs.
+    uint32_t qb[kNT][kKSteps][2];
+    float qs[kNT][2];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      const bool real = nt * 8 + r < group;
+      const T* qrow = static_cast<const T*>(p.q) + b * p.q_stride +
+                      static_cast<int64_t>(h * group + (real ? nt * 8 + r : 0)) * D + 4 * q4;
+      float2 x[kKSteps][2];
+      float mx = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < kKSteps; ++kk) {
+        const uint2 v = real ? *reinterpret_cast<const uint2*>(qrow + 16 * kk) : make_uint2(0u, 0u);
+        x[kk][0] = unpack2<T>(v.x);
+        x[kk][1] = unpack2<T>(v.y);
+        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[kk][0].x), fabsf(x[kk][0].y)),
+                             fmaxf(fabsf(x[kk][1].x), fabsf(x[kk][1].y))));
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // Exponent of the head's largest |q|, clamped so that 2^-e is a normal number.
+      const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23) - 127, -120), 120);
+      const float down = pow2f(-e);
+#pragma unroll
+      for (int kk = 0; kk < kKSteps; ++kk) {
+        qb[nt][kk][0] = pack2<__half>(x[kk][0].x * down, x[kk][0].y * down);
+        qb[nt][kk][1] = pack2<__half>(x[kk][1].x * down, x[kk][1].y * down);
+      }
+      const float up = p.scale_log2 * pow2f(e);
+      qs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * q4);      // a lane of head 2 q4
+      qs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * q4 + 4);  // a lane of head 2 q4 + 1
+    }
+
+    float o[kNT][kKSteps][4];  // [dims 16 kk + 2 r (+1)][heads 2 q4, 2 q4 + 1]: {d0h0, d0h1, d1h0, d1h1}
+    // Per head: running maxima of s (m) and s + log2 b (mv), the factor of P'
+    // 2^(m - mv + 7), and this lane's part of the softmax sum.
+    float m[kNT][2], mv[kNT][2], f[kNT][2], l[kNT][2];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+      for (int kk = 0; kk < kKSteps; ++kk) o[nt][kk][0] = o[nt][kk][1] = o[nt][kk][2] = o[nt][kk][3] = 0.f;
+      m[nt][0] = m[nt][1] = mv[nt][0] = mv[nt][1] = -INFINITY;
+      f[nt][0] = f[nt][1] = l[nt][0] = l[nt][1] = 0.f;
+    }
+    int stuck_at = -1;
+
+    const int row8 = (lane & 7) + ((lane >> 3) & 1) * 8;  // ldmatrix: row of this lane's address
+    const int chunk1 = lane >> 4;                         // and its 16-byte chunk (0 or 1)
+
+    for (int it = 0; warp + it * NW < nchunk; ++it) {
+      const int j = warp + it * NW;
+      const int st = warp * NS + (gbase + it) % NS;
+      if (!mbar_wait_bounded(&bars[st], ((gbase + it) / NS) & 1)) {
+        stuck_at = it;
+        break;
+      }
+      const uint32_t kbase = smem_u32(smem + st * 2 * SM::kTileBytes);
+      const uint32_t vbase = kbase + SM::kTileBytes;
+      const float* ks = reinterpret_cast<const float*>(smem + SM::kScaleOffset + st * 2 * kKeys * 4);
+      const int left = n_keys - j * kKeys;  // keys of the partition from this stage on
+
+      // ---- S^T: two key tiles of 16
+      float s[2][kNT][4];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) s[kt][nt][0] = s[kt][nt][1] = s[kt][nt][2] = s[kt][nt][3] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < kKSteps; kk += 2) {
+          uint32_t w[4];
+          ldsm_x4(kbase + SM::off(kt * 16 + row8, kk + chunk1), w[0], w[1], w[2], w[3]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t a0, a1, a2, a3;
+            decode4<C>(w[2 * x], a0, a2);
+            decode4<C>(w[2 * x + 1], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+              Mma<__half>::run(s[kt][nt], a0, a1, a2, a3, qb[nt][kk + x][0], qb[nt][kk + x][1]);
+          }
+        }
+      }
+
+      // ---- scores in log2 units; this lane's keys are r, r + 8, r + 16, r + 24
+      float vs[4];
+      float top[kNT][2], topv[kNT][2];
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) top[nt][0] = top[nt][1] = topv[nt][0] = topv[nt][1] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = r + 8 * i;
+        const bool live = key < left;
+        const float a = ks[key];
+        vs[i] = live ? ks[kKeys + key] : 0.f;
+        // log2 b to within 0.09: the bits of a float, read as an integer, are linear
+        // in its logarithm between powers of two. Only the choice of M uses it.
+        const float lb = fmaf(static_cast<float>(__float_as_int(vs[i])), 0x1p-23f, -127.f);
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& x = s[i >> 1][nt][(i & 1) * 2 + e];
+            x = live ? x * (a * qs[nt][e]) : -INFINITY;
+            top[nt][e] = fmaxf(top[nt][e], x);
+            topv[nt][e] = fmaxf(topv[nt][e], x + lb);
+          }
+        }
+      }
+      // ---- running maxima, moved only when passed by 2^8
+      bool move = false;
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          move |= top[nt][e] > m[nt][e] + 8.f || topv[nt][e] > mv[nt][e] + 8.f;
+      }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          float alpha[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float t = top[nt][e], u = topv[nt][e];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+              u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, x));
+            }
+            const float m_new = fmaxf(m[nt][e], t);
+            const float mv_new = fmaxf(mv[nt][e], u);
+            l[nt][e] *= m_new == -INFINITY ? 1.f : ex2(m[nt][e] - m_new);
+            alpha[e] = mv_new == -INFINITY ? 1.f : ex2(mv[nt][e] - mv_new);
+            m[nt][e] = m_new;
+            mv[nt][e] = mv_new;
+            f[nt][e] = ex2(fminf(m_new - mv_new + 7.f, 120.f));
+          }
+#pragma unroll
+          for (int kk = 0; kk < kKSteps; ++kk) {
+            o[nt][kk][0] *= alpha[0];
+            o[nt][kk][1] *= alpha[1];
+            o[nt][kk][2] *= alpha[0];
+            o[nt][kk][3] *= alpha[1];
+          }
+        }
+      }
+
+      // ---- P^T as the B operand: [kt][nt][keys 0-7 | 8-15]
+      uint32_t pb[2][kNT][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          const float p0 = ex2(s[i >> 1][nt][(i & 1) * 2] - m[nt][0]);
+          const float p1 = ex2(s[i >> 1][nt][(i & 1) * 2 + 1] - m[nt][1]);
+          l[nt][0] += p0;
+          l[nt][1] += p1;
+          pb[i >> 1][nt][i & 1] = transpose8x8(pack2<__half>(p0 * (vs[i] * f[nt][0]), p1 * (vs[i] * f[nt][1])));
+        }
+      }
+
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        // Codes of keys past the end become 0: what a block holds there (NaN codes
+        // among it) must not meet a probability of 0. This lane's keys are
+        // 2 q4, 2 q4 + 1 (low and high half of a register) and the same plus 8.
+        uint32_t live0 = 0xffffffffu, live1 = 0xffffffffu;
+        if (left < kKeys) {
+          const int k0 = left - kt * 16 - 2 * q4;
+          live0 = k0 >= 2 ? 0xffffffffu : k0 == 1 ? 0x0000ffffu : 0u;
+          live1 = k0 >= 10 ? 0xffffffffu : k0 == 9 ? 0x0000ffffu : 0u;
+        }
+#pragma unroll
+        for (int kk = 0; kk < kKSteps; kk += 2) {
+          uint32_t w[4];
+          ldsm_x4_t(vbase + SM::off(kt * 16 + row8, kk + chunk1), w[0], w[1], w[2], w[3]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            // bytes (key0 dim0, key0 dim1, key1 dim0, key1 dim1) -> pairs of keys per dim
+            uint32_t a0, a1, a2, a3;
+            decode4<C>(__byte_perm(w[2 * x] & live0, 0, 0x3120), a0, a1);
+            decode4<C>(__byte_perm(w[2 * x + 1] & live1, 0, 0x3120), a2, a3);
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+              Mma<__half>::run(o[nt][kk + x], a0, a1, a2, a3, pb[kt][nt][0], pb[kt][nt][1]);
+          }
+        }
+      }
+
+      __syncwarp();
+      if (warp + (it + NS) * NW < nchunk) {
+        fence_proxy_async_smem();  // our reads of this stage precede the refill
+        issue(it + NS);
+      }
+    }
+
+    if (stuck_at >= 0) {
+      set_device_error(p.err, PS_DEVERR_TIMEOUT);
+      // Drain this warp's copies still in flight, each wait bounded.
+      if (lane == 0) {
+        for (int x = 0; x < NS; ++x) {
+          const int i2 = stuck_at + x;
+          if (warp + i2 * NW < nchunk)
+            (void)mbar_wait_bounded(&bars[warp * NS + (gbase + i2) % NS], ((gbase + i2) / NS) & 1);
+        }
+      }
+    }
+    __syncwarp();
+
+    // ---- merge the warps through shared memory
+    __syncthreads();  // every warp is done reading its ring; alias it as the merge area
+    float* ms = reinterpret_cast<float*>(smem);  // [NW][R]
+    float* ls = ms + NW * R;                     // [NW][R]
+    float* os = ls + NW * R;                     // [NW][R][D]
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float t = l[nt][e];  // each lane summed its own keys
+        t += __shfl_xor_sync(0xffffffffu, t, 4);
+        t += __shfl_xor_sync(0xffffffffu, t, 8);
+        t += __shfl_xor_sync(0xffffffffu, t, 16);
+        const int head = nt * 8 + 2 * q4 + e;
+        const float unit = f[nt][e] > 0.f ? 1.f / f[nt][e] : 0.f;  // O / f is in units of 2^m, like l
+        if (r == 0) {
+          ms[warp * R + head] = m[nt][e];
+          ls[warp * R + head] = t;
+        }
+#pragma unroll
+        for (int kk = 0; kk < kKSteps; ++kk)
+          *reinterpret_cast<float2*>(&os[(warp * R + head) * D + 16 * kk + 2 * r]) =
+              make_float2(o[nt][kk][e] * unit, o[nt][kk][2 + e] * unit);
+      }
+    }
+    __syncthreads();
+
+    const bool single = nsplit == 1;
+    for (int idx = threadIdx.x; idx < group * (D / 4); idx += blockDim.x) {
+      const int g = idx / (D / 4);
+      const int d = (idx % (D / 4)) * 4;
+      float mmax = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) mmax = fmaxf(mmax, ms[w * R + g]);
+      float lsum = 0.f;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float mw = ms[w * R + g];
+        const float sc = (mw == -INFINITY) ? 0.f : exp2f(mw - mmax);
+        lsum += ls[w * R + g] * sc;
+        const float4 ov = *reinterpret_cast<const float4*>(&os[(w * R + g) * D + d]);
+        acc[0] += ov.x * sc;
+        acc[1] += ov.y * sc;
+        acc[2] += ov.z * sc;
+        acc[3] += ov.w * sc;
+      }
+      // lsum is positive for finite scores; a NaN score leaves it NaN, and the output with it
+      const float inv = 1.f / lsum;
+      const int qh = h * group + g;
+      if (single) {
+        T* orow = static_cast<T*>(p.out) + b * p.out_stride + static_cast<int64_t>(qh) * D + d;
+        uint2 packed;
+        packed.x = pack2<T>(acc[0] * inv, acc[1] * inv);
+        packed.y = pack2<T>(acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<uint2*>(orow) = packed;
+      } else {
+        const int64_t slot = (static_cast<int64_t>(b) * p.max_splits + split) * p.num_q_heads + qh;
+        *reinterpret_cast<float4*>(p.ws_o + slot * D + d) =
+            make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+        if (d == 0) p.ws_lse[slot] = mmax + log2f(lsum);
+      }
+    }
+    gbase += nchunk > warp ? static_cast<uint32_t>((nchunk - warp + NW - 1) / NW) : 0u;
+    if constexpr (kList) {
+      // The merge area aliases the ring: every thread is done with it before the
+      // next unit's copies write it.
+      fence_proxy_async_smem();
+      __syncthreads();
+    }
+  }
+}
+
+// ------------------------------------------------------------ host side
+constexpr int kNW = 4;  // warps per CTA
+constexpr int kNS = 2;  // stages of 32 keys per warp
+
+template <typename T, typename C, int D, int BS, int R>
+int launch_quant(const QuantDecodeParams& qp, const CUtensorMap& km, const CUtensorMap& vm,
+                 cudaStream_t s) {
+  const DecodeParams& p = qp.d;
+  using SM = QuantSmem<D, kNW, kNS>;
+  const size_t smem = SM::bytes(p.table_cap);
+  const char* fn = "ps_paged_decode_quant";
+  if (p.max_splits <= 1) {
+    auto kern = paged_decode_quant_kernel<T, C, D, kNW, kNS, BS, R, false>;
+    static size_t configured[64] = {};
+    int st = reserve_smem(kern, smem, configured);
+    if (st != PS_OK) return st;
+    const cudaError_t e = launch_pdl(kern, dim3(p.num_kv_heads, 1, p.num_launch), dim3(kNW * 32),
+                                     smem, s, qp, km, vm);
+    if (e != cudaSuccess) return fail(PS_ERR_CUDA, "%s: launch failed: %s", fn, cudaGetErrorString(e));
+    return check_launch(fn);
+  }
+  auto kern = paged_decode_quant_kernel<T, C, D, kNW, kNS, BS, R, true>;
+  static size_t configured[64] = {};
+  int st = reserve_smem(kern, smem, configured);
+  if (st != PS_OK) return st;
+  int dev = 0, sms = 148, per_sm = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kNW * 32, smem);
+  if (e != cudaSuccess || per_sm <= 0)
+    return fail(PS_ERR_CUDA, "%s: occupancy query failed: %s", fn, cudaGetErrorString(e));
+  if (!p.planned) {
+    e = launch_pdl(decode_plan_kernel, dim3(1), dim3(1024), 0, s, p);
+    if (e != cudaSuccess)
+      return fail(PS_ERR_CUDA, "%s(plan): launch failed: %s", fn, cudaGetErrorString(e));
+  }
+  e = launch_pdl(kern, dim3(per_sm * sms), dim3(kNW * 32), smem, s, qp, km, vm);
+  if (e != cudaSuccess) return fail(PS_ERR_CUDA, "%s: launch failed: %s", fn, cudaGetErrorString(e));
+  const int warps = p.num_launch * p.num_q_heads;
+  e = launch_pdl(decode_combine_kernel<T, D>, dim3((warps + 3) / 4), dim3(128), 0, s, p);
+  if (e != cudaSuccess)
+    return fail(PS_ERR_CUDA, "%s(combine): launch failed: %s", fn, cudaGetErrorString(e));
+  return check_launch(fn);
+}
+
+template <typename T, typename C, int D>
+int dispatch_geometry(const QuantDecodeParams& p, const CUtensorMap& km, const CUtensorMap& vm,
+                      cudaStream_t s) {
+  const bool wide = p.d.group > 8;
+  if (p.d.block_size == 8)
+    return wide ? launch_quant<T, C, D, 8, 16>(p, km, vm, s) : launch_quant<T, C, D, 8, 8>(p, km, vm, s);
+  if (p.d.block_size == 32)
+    return wide ? launch_quant<T, C, D, 32, 16>(p, km, vm, s) : launch_quant<T, C, D, 32, 8>(p, km, vm, s);
+  return wide ? launch_quant<T, C, D, 16, 16>(p, km, vm, s) : launch_quant<T, C, D, 16, 8>(p, km, vm, s);
+}
+
+template <typename T>
+int dispatch_code(const QuantDecodeParams& p, const CUtensorMap& km, const CUtensorMap& vm,
+                  cudaStream_t s, int code, int head_dim) {
+  if (code == PS_CODE_E4M3)
+    return head_dim == 128 ? dispatch_geometry<T, CodeE4M3, 128>(p, km, vm, s)
+                           : dispatch_geometry<T, CodeE4M3, 64>(p, km, vm, s);
+  return head_dim == 128 ? dispatch_geometry<T, CodeInt8, 128>(p, km, vm, s)
+                         : dispatch_geometry<T, CodeInt8, 64>(p, km, vm, s);
+}
+
+}  // namespace
+}  // namespace ps
+
+using namespace ps;
+
+extern "C" int ps_paged_decode_quant(
+    void* out, int64_t out_seq_stride, const void* query, int64_t query_seq_stride,
+    const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
+    int64_t num_blocks, const int32_t* block_tables, int64_t block_table_stride,
+    const int32_t* ctx_lens, int num_seqs, const int32_t* seq_list, int num_listed, int num_q_heads,
+    int num_kv_heads, int head_dim, int block_size, int max_blocks_per_seq, float scale,
+    int split_tokens, int planned, void* workspace, int64_t workspace_bytes, int dtype, int code,
+    int32_t* device_error, void* stream) {
+  ps::NvtxRange nvtx_range("ps_paged_decode_quant");
+  const char* fn = "ps_paged_decode_quant";
+  if (code != PS_CODE_E4M3 && code != PS_CODE_INT8)
+    return fail(PS_ERR_UNSUPPORTED, "%s: code %d unsupported (e4m3 or int8)", fn, code);
+  int part = 0, max_splits = 0, table_cap = 0;
+  int st = validate_decode(fn, out, out_seq_stride, query, query_seq_stride, k_pool, v_pool,
+                           num_blocks, block_tables, block_table_stride, ctx_lens, num_seqs,
+                           num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                           split_tokens, dtype, &part, &max_splits, &table_cap);
+  if (st != PS_OK || num_seqs == 0) return st;
+  if (!k_scale || !v_scale || !aligned(k_scale, 16) || !aligned(v_scale, 16))
+    return fail(PS_ERR_INVALID, "%s: k_scale/v_scale must be 16-byte aligned device pointers", fn);
+  if (num_listed > num_seqs || (num_listed > 0 && !seq_list))
+    return fail(PS_ERR_INVALID, "%s: num_listed %d needs a list of at most num_seqs %d entries", fn,
+                num_listed, num_seqs);
+  if (num_listed == 0) return PS_OK;
+  QuantDecodeParams qp{};
+  DecodeParams& p = qp.d;
+  if (max_splits > 1) {
+    st = set_split_workspace(fn, &p, num_seqs, num_q_heads, head_dim, block_size,
+                             max_blocks_per_seq, split_tokens, max_splits, workspace,
+                             workspace_bytes);
+    if (st != PS_OK) return st;
+  }
+  p.out = out;
+  p.q = query;
+  p.out_stride = out_seq_stride;
+  p.q_stride = query_seq_stride;
+  p.block_tables = block_tables;
+  p.bt_stride = block_table_stride;
+  p.ctx_lens = ctx_lens;
+  p.num_blocks = num_blocks;
+  p.num_seqs = num_seqs;
+  p.num_launch = num_listed < 0 ? num_seqs : num_listed;
+  p.planned = planned != 0;
+  p.num_q_heads = num_q_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.group = num_q_heads / num_kv_heads;
+  p.max_blocks = max_blocks_per_seq;
+  p.block_size = block_size;
+  p.part_tokens = part;
+  p.max_splits = max_splits;
+  p.table_cap = table_cap;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.err = device_error;
+  p.seq_order = seq_list;
+  qp.k_scale = k_scale;
+  qp.v_scale = v_scale;
+  const uint64_t rows = static_cast<uint64_t>(num_blocks) * num_kv_heads * block_size;
+  CUtensorMap km, vm;
+  const int box = block_size < kKeys ? block_size : kKeys;
+  st = get_pool_tmap(k_pool, rows, head_dim, box, &km, 1);
+  if (st != PS_OK) return st;
+  st = get_pool_tmap(v_pool, rows, head_dim, box, &vm, 1);
+  if (st != PS_OK) return st;
+  cudaStream_t s = as_stream(stream);
+  return dtype == PS_DTYPE_BF16 ? dispatch_code<__nv_bfloat16>(qp, km, vm, s, code, head_dim)
+                                : dispatch_code<__half>(qp, km, vm, s, code, head_dim);
+}

@@ -10,6 +10,7 @@ KV pool layout (per layer): ``[num_blocks, num_kv_heads, block_size, head_dim]``
 
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -19,17 +20,24 @@ from paged_serve_b200 import _lib
 __all__ = [
     "build_slot_mapping",
     "cache_append",
+    "cache_append_quant",
     "cache_append_rope",
+    "cache_append_rope_quant",
+    "cache_read_quant",
     "copy_blocks",
     "check_block_pairs",
     "decode_plan",
     "decode_workspace_bytes",
     "paged_decode",
     "paged_decode_listed",
+    "paged_decode_quant",
     "paged_prefill",
     "stream_read",
     "swap_blocks",
 ]
+
+# Code types of an 8-bit cache.
+CODES = {torch.float8_e4m3fn: _lib.PS_CODE_E4M3, torch.int8: _lib.PS_CODE_INT8}
 
 _DTYPES = {torch.bfloat16: _lib.PS_DTYPE_BF16, torch.float16: _lib.PS_DTYPE_F16}
 
@@ -58,6 +66,13 @@ def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
 
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def _on(device: torch.device):
+    """Makes ``device`` current for a launch (a no-op where it already is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -164,6 +179,155 @@ def cache_append_rope(
         _err_ptr(device_error), _stream(dev),
     )
     _lib.check(st, "cache_append_rope")
+
+
+def _check_quant_pools(k_pool, v_pool, k_scale, v_scale) -> int:
+    """Checks an 8-bit cache's pools and scales; returns their code type."""
+    _check_pool(k_pool, "k_pool")
+    _check_pool(v_pool, "v_pool")
+    if k_pool.dtype not in CODES:
+        raise ValueError(f"an 8-bit cache holds float8_e4m3fn or int8 codes, not {k_pool.dtype}")
+    if v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype:
+        raise ValueError("k_pool/v_pool must share shape and dtype")
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if t.dtype != torch.float32 or t.shape != k_pool.shape[:3] or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 [num_blocks, kv_heads, block_size]")
+    return CODES[k_pool.dtype]
+
+
+def _append_quant(what, k_pool, v_pool, k_scale, v_scale, key, value, slot_mapping, positions,
+                  cos_sin_table, device_error) -> None:
+    dev = _require_cuda(k_pool, v_pool, k_scale, v_scale, key, value, slot_mapping, positions,
+                        cos_sin_table, device_error)
+    code = _check_quant_pools(k_pool, v_pool, k_scale, v_scale)
+    nb, hkv, bs, d = k_pool.shape
+    if key.dtype != value.dtype:
+        raise ValueError("key/value must share a dtype")
+    ks = _check_rows(key, "key", hkv, d)
+    vs = _check_rows(value, "value", hkv, d)
+    t = key.shape[0]
+    if value.shape[0] != t or slot_mapping.shape != (t,) or slot_mapping.dtype != torch.int64:
+        raise ValueError("slot_mapping must be int64 [num_tokens] matching key/value")
+    if not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous")
+    pools = (k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+             key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr())
+    geometry = (t, ks, vs, hkv, d, bs, nb)
+    tail = (_dtype_code(key), code, _err_ptr(device_error), _stream(dev))
+    lib = _lib.load()
+    with _on(dev):
+        if positions is None:
+            st = lib.ps_cache_append_quant(*pools, *geometry, *tail)
+        else:
+            if positions.shape != (t,) or positions.dtype != torch.int64 or \
+                    not positions.is_contiguous():
+                raise ValueError("positions must be contiguous int64 [num_tokens]")
+            if (cos_sin_table.dim() != 2 or cos_sin_table.shape[1] != d
+                    or cos_sin_table.dtype != key.dtype or not cos_sin_table.is_contiguous()):
+                raise ValueError(f"cos_sin_table must be contiguous [positions, {d}] of the key dtype")
+            st = lib.ps_cache_append_rope_quant(
+                *pools, positions.data_ptr(), *geometry, cos_sin_table.data_ptr(),
+                cos_sin_table.shape[0], d, *tail)
+    _lib.check(st, what)
+
+
+def cache_append_quant(
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    device_error: torch.Tensor | None = None,
+) -> None:
+    """:func:`cache_append` into an 8-bit cache: quantises each row as it is written.
+
+    The pools hold codes (``float8_e4m3fn`` or ``int8``), ``k_scale``/``v_scale`` one
+    float32 scale per row (``[num_blocks, Hkv, block_size]``). For a row x,
+    ``scale = max(max|x| / qmax, 2**-126)`` (qmax 448 or 127) and
+    ``code = round(x * (1 / scale))``, each step in float32; the value is
+    ``code * scale``. The reference's cache holds the model's dtype and has no counterpart.
+    """
+    _append_quant("cache_append_quant", k_pool, v_pool, k_scale, v_scale, key, value,
+                  slot_mapping, None, None, device_error)
+
+
+def cache_append_rope_quant(
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    positions: torch.Tensor,
+    cos_sin_table: torch.Tensor,
+    device_error: torch.Tensor | None = None,
+) -> None:
+    """:func:`cache_append_quant` with split-half RoPE applied to K on the way in.
+
+    K is rotated in float32 with ``cos_sin_table`` (:func:`paged_serve_b200.rope.cos_sin_table`,
+    in the key's dtype) and quantised from there, without the roundings to the
+    storage type that :func:`cache_append_rope` makes.
+    """
+    if positions is None or cos_sin_table is None:
+        raise ValueError("cache_append_rope_quant needs positions and cos_sin_table")
+    _append_quant("cache_append_rope_quant", k_pool, v_pool, k_scale, v_scale, key, value,
+                  slot_mapping, positions, cos_sin_table, device_error)
+
+
+def cache_read_quant(
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_tables: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    k_out: torch.Tensor,
+    v_out: torch.Tensor,
+    out_tables: torch.Tensor,
+    device_error: torch.Tensor | None = None,
+) -> None:
+    """Tokens ``[0, ctx_lens[b])`` of each sequence back from an 8-bit cache.
+
+    Block j of sequence b goes from pool block ``block_tables[b, j]`` to block
+    ``out_tables[b, j]`` of the bf16/fp16 pools ``k_out``/``v_out`` (same heads, block
+    size and head dim, any number of blocks) as ``code * scale``, rounded once; rows
+    past the last token become zeros and other blocks stay as they are.
+    :func:`paged_prefill` and :func:`paged_decode_shared` run on the result with
+    ``out_tables``.
+    """
+    dev = _require_cuda(k_pool, v_pool, k_scale, v_scale, block_tables, ctx_lens, k_out, v_out,
+                        out_tables, device_error)
+    code = _check_quant_pools(k_pool, v_pool, k_scale, v_scale)
+    _check_pool(k_out, "k_out")
+    _check_pool(v_out, "v_out")
+    nb, hkv, bs, d = k_pool.shape
+    if k_out.shape[1:] != k_pool.shape[1:] or v_out.shape != k_out.shape or \
+            v_out.dtype != k_out.dtype:
+        raise ValueError("k_out/v_out must share shape and dtype and match the pools' block shape")
+    b = ctx_lens.shape[0]
+    if ctx_lens.dtype != torch.int32 or ctx_lens.shape != (b,) or not ctx_lens.is_contiguous():
+        raise ValueError("ctx_lens must be contiguous int32 [num_seqs]")
+    for t, name in ((block_tables, "block_tables"), (out_tables, "out_tables")):
+        if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != b or \
+                t.shape[1] != block_tables.shape[1]:
+            raise ValueError(f"{name} must be int32 [num_seqs, max_blocks]")
+        if t.stride(1) != 1:
+            raise ValueError(f"{name} rows must be contiguous")
+    w = block_tables.shape[1]
+    if b == 0 or w == 0:
+        return
+    with _on(dev):
+        st = _lib.load().ps_cache_read_quant(
+            k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nb,
+            k_out.data_ptr(), v_out.data_ptr(), k_out.shape[0], block_tables.data_ptr(),
+            block_tables.stride(0) if b > 1 else w, out_tables.data_ptr(),
+            out_tables.stride(0) if b > 1 else w, ctx_lens.data_ptr(), b, hkv, d, bs, w,
+            _dtype_code(k_out), code, _err_ptr(device_error), _stream(dev),
+        )
+    _lib.check(st, "cache_read_quant")
 
 
 def check_block_pairs(pairs) -> None:
@@ -376,14 +540,14 @@ class _DecodeArgs:
     """Validated arguments shared by :func:`paged_decode` and :func:`paged_decode_append`."""
 
     def __init__(self, query, k_pool, v_pool, block_tables, ctx_lens, out, workspace,
-                 device_error, seq_order, *extra):
+                 device_error, seq_order, *extra, quantised=False):
         self.dev = _require_cuda(query, k_pool, v_pool, block_tables, ctx_lens, out, workspace,
                                  device_error, seq_order, *extra)
         _check_pool(k_pool, "k_pool")
         _check_pool(v_pool, "v_pool")
         self.nb, self.hkv, self.bs, self.d = k_pool.shape
         d = self.d
-        if v_pool.shape != k_pool.shape or query.dtype != k_pool.dtype:
+        if v_pool.shape != k_pool.shape or (query.dtype != k_pool.dtype and not quantised):
             raise ValueError("k_pool/v_pool/query must share shape and dtype")
         if query.dim() != 3:
             raise ValueError("query must be [num_seqs, num_q_heads, head_dim]")
@@ -479,6 +643,55 @@ def paged_decode_listed(
         _stream(a.dev),
     )
     _lib.check(st, "paged_decode_listed")
+    return a.out
+
+
+def paged_decode_quant(
+    query: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_tables: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    scale: float,
+    split_tokens: int = 0,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    device_error: torch.Tensor | None = None,
+    seq_order: torch.Tensor | None = None,
+    planned: bool = False,
+    seq_list: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_decode` over an 8-bit cache (:func:`cache_append_quant`).
+
+    ``query``/``out`` are bf16 or fp16, the pools ``float8_e4m3fn`` or ``int8`` codes with
+    their scales. ``split_tokens``, ``workspace`` (:func:`decode_workspace_bytes`) and
+    ``seq_order`` as in :func:`paged_decode`; ``planned``: the split-K unit list of
+    these lengths is already in ``workspace`` (:func:`decode_plan`); ``seq_list``: only
+    these sequences, as in :func:`paged_decode_listed` (not with ``seq_order`` or
+    ``planned``). Keys past a sequence's length are ignored whatever their rows hold.
+    """
+    a = _DecodeArgs(query, k_pool, v_pool, block_tables, ctx_lens, out, workspace, device_error,
+                    seq_order, seq_list, k_scale, v_scale, quantised=True)
+    code = _check_quant_pools(k_pool, v_pool, k_scale, v_scale)
+    listed, list_ptr = -1, a.order_ptr
+    if seq_list is not None:
+        if seq_order is not None or planned:
+            raise ValueError("seq_list cannot be combined with seq_order or planned")
+        if seq_list.dtype != torch.int32 or seq_list.dim() != 1 or not seq_list.is_contiguous():
+            raise ValueError("seq_list must be contiguous int32 [n]")
+        listed = seq_list.shape[0]
+        list_ptr = seq_list.data_ptr() if listed else None
+    with _on(a.dev):
+        st = _lib.load().ps_paged_decode_quant(
+            a.out.data_ptr(), a.os, query.data_ptr(), a.qs, k_pool.data_ptr(), v_pool.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), a.nb, block_tables.data_ptr(), a.bt_stride,
+            ctx_lens.data_ptr(), a.b, list_ptr, listed, a.hq, a.hkv, a.d, a.bs, a.max_blocks,
+            float(scale), int(split_tokens), int(planned), a.ws_ptr, a.ws_bytes,
+            _dtype_code(query), code, _err_ptr(device_error), _stream(a.dev),
+        )
+    _lib.check(st, "paged_decode_quant")
     return a.out
 
 

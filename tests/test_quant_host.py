@@ -1,0 +1,119 @@
+"""Refusals of the 8-bit cache's entry points, on the host, before any launch."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from paged_serve_b200 import _lib, ops
+
+
+def _msg():
+    return _lib.load().ps_last_error_string().decode()
+
+
+def _append(**kw):
+    a = dict(t=4, ks=256, vs=256, hkv=2, d=128, bs=16, nb=8, dtype=2, code=1, pool=16, rope=False)
+    a.update(kw)
+    lib = _lib.load()
+    head = [a["pool"], 16, 16, 16, 16, 16, 16]
+    geo = [a["t"], a["ks"], a["vs"], a["hkv"], a["d"], a["bs"], a["nb"]]
+    if a["rope"]:
+        return lib.ps_cache_append_rope_quant(*head, a.get("pos", 16), *geo, a.get("table", 16), 10,
+                                              a.get("rope_dim", a["d"]), a["dtype"], a["code"], None, None)
+    return lib.ps_cache_append_quant(*head, *geo, a["dtype"], a["code"], None, None)
+
+
+def test_append_refusals():
+    assert _append(dtype=3) == _lib.PS_ERR_UNSUPPORTED and "dtype" in _msg()
+    assert _append(code=3) == _lib.PS_ERR_UNSUPPORTED and "code" in _msg()
+    assert _append(d=96) == _lib.PS_ERR_UNSUPPORTED
+    assert _append(t=-1) == _lib.PS_ERR_INVALID
+    assert _append(t=0) == _lib.PS_OK
+    assert _append(pool=None) == _lib.PS_ERR_INVALID
+    assert _append(pool=8) == _lib.PS_ERR_INVALID and "aligned" in _msg()
+    assert _append(ks=128) == _lib.PS_ERR_INVALID
+    assert _append(ks=260) == _lib.PS_ERR_INVALID
+    assert _append(nb=1 << 40) == _lib.PS_ERR_INVALID
+    assert _append(t=1 << 60) == _lib.PS_ERR_INVALID
+    assert _append(rope=True, rope_dim=64) == _lib.PS_ERR_UNSUPPORTED
+    assert _append(rope=True, table=None) == _lib.PS_ERR_INVALID
+    assert _append(rope=True, pos=None) == _lib.PS_ERR_INVALID
+
+
+def _read(**kw):
+    a = dict(nb=8, onb=8, ts=4, ots=4, b=2, hkv=2, d=128, bs=16, mb=4, dtype=2, code=2, out=16)
+    a.update(kw)
+    return _lib.load().ps_cache_read_quant(16, 16, 16, 16, a["nb"], a["out"], 16, a["onb"], 16, a["ts"], 16,
+                                           a["ots"], 16, a["b"], a["hkv"], a["d"], a["bs"], a["mb"],
+                                           a["dtype"], a["code"], None, None)
+
+
+def test_read_refusals():
+    assert _read(dtype=0) == _lib.PS_ERR_UNSUPPORTED
+    assert _read(code=0) == _lib.PS_ERR_UNSUPPORTED
+    assert _read(d=32) == _lib.PS_ERR_UNSUPPORTED
+    assert _read(b=0) == _lib.PS_OK
+    assert _read(b=70000) == _lib.PS_ERR_INVALID
+    assert _read(onb=0) == _lib.PS_ERR_INVALID
+    assert _read(ts=3) == _lib.PS_ERR_INVALID
+    assert _read(ots=3) == _lib.PS_ERR_INVALID
+    assert _read(out=None) == _lib.PS_ERR_INVALID
+    assert _read(out=24) == _lib.PS_ERR_INVALID
+    assert _read(mb=1 << 28, ts=1 << 28, ots=1 << 28) == _lib.PS_ERR_INVALID
+
+
+def _decode(**kw):
+    a = dict(os=1024, qs=1024, ks=16, nb=8, bts=4, b=2, order=None, listed=-1, hq=8, hkv=2, d=128, bs=16, mb=4,
+             split=0, ws=None, wsb=0, dtype=2, code=1)
+    a.update(kw)
+    return _lib.load().ps_paged_decode_quant(
+        16, a["os"], 16, a["qs"], 16, 16, a["ks"], 16, a["nb"], 16, a["bts"], 16, a["b"], a["order"],
+        a["listed"], a["hq"], a["hkv"], a["d"], a["bs"], a["mb"], 0.1, a["split"], 0, a["ws"], a["wsb"],
+        a["dtype"], a["code"], None, None)
+
+
+def test_decode_refusals():
+    assert _decode(code=7) == _lib.PS_ERR_UNSUPPORTED
+    assert _decode(dtype=7) == _lib.PS_ERR_UNSUPPORTED
+    assert _decode(d=256) == _lib.PS_ERR_UNSUPPORTED
+    assert _decode(bs=4) == _lib.PS_ERR_UNSUPPORTED
+    assert _decode(hq=34, os=34 * 128, qs=34 * 128) == _lib.PS_ERR_UNSUPPORTED
+    assert _decode(hq=9) == _lib.PS_ERR_INVALID
+    assert _decode(ks=None) == _lib.PS_ERR_INVALID and "scale" in _msg()
+    assert _decode(ks=20) == _lib.PS_ERR_INVALID
+    assert _decode(listed=1) == _lib.PS_ERR_INVALID
+    assert _decode(listed=3, order=16) == _lib.PS_ERR_INVALID
+    assert _decode(listed=0) == _lib.PS_OK
+    assert _decode(b=0) == _lib.PS_OK
+    assert _decode(split=24) == _lib.PS_ERR_INVALID
+    assert _decode(split=16) == _lib.PS_ERR_INVALID and "workspace" in _msg()
+    assert _decode(split=16, ws=256, wsb=100) == _lib.PS_ERR_INVALID
+
+
+def test_ops_refuse_host_tensors():
+    kp = torch.zeros((2, 1, 16, 64), dtype=torch.int8)
+    sc = torch.zeros((2, 1, 16))
+    x = torch.zeros((1, 1, 64), dtype=torch.bfloat16)
+    slots = torch.zeros(1, dtype=torch.int64)
+    tables = torch.zeros((1, 2), dtype=torch.int32)
+    n = torch.ones(1, dtype=torch.int32)
+    out = torch.zeros((2, 1, 16, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.cache_append_quant(kp, kp, sc, sc, x, x, slots)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.cache_read_quant(kp, kp, sc, sc, tables, n, out, out, tables)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.paged_decode_quant(x, kp, kp, sc, sc, tables, n, 1.0)
+
+
+def test_quant_pools_are_checked():
+    kp = torch.zeros((2, 1, 16, 64), dtype=torch.int8)
+    sc = torch.zeros((2, 1, 16))
+    assert ops._check_quant_pools(kp, kp, sc, sc) == _lib.PS_CODE_INT8
+    f8 = kp.view(torch.float8_e4m3fn)
+    assert ops._check_quant_pools(f8, f8, sc, sc) == _lib.PS_CODE_E4M3
+    for bad in ((kp.to(torch.uint8), kp, sc, sc), (kp, f8, sc, sc), (kp, kp[:1], sc, sc), (kp, kp, sc[:1], sc),
+                (kp, kp, sc, sc.double()), (kp, kp, sc.transpose(0, 2), sc), (kp[0], kp, sc, sc)):
+        with pytest.raises(ValueError):
+            ops._check_quant_pools(*bad)
