@@ -468,6 +468,50 @@ PS_API int64_t ps_paged_prefill_workspace_bytes(int num_seqs, int max_q_len, int
                                                 int max_blocks_per_seq, int split_keys);
 
 /*
+ * ps_paged_decode_shared — ps_paged_decode where groups of neighbouring sequences
+ * share their leading blocks: each group's shared prefix is read once for all its
+ * rows (on tcgen05 tensor cores, as in ps_paged_prefill), the keys behind it as in
+ * ps_paged_decode, and both are merged by their log-sum-exps. No counterpart in the
+ * reference (a prefix cache is planned there, AGENTS.md; its decode is one SDPA).
+ *
+ * Arguments as ps_paged_decode_ordered, and:
+ * group_starts: [num_groups + 1] int32, group g = batch rows
+ *   [group_starts[g], group_starts[g + 1]); at most max_group rows each.
+ * shared_lens: [num_seqs] int32, the shared keys of each row: a multiple of
+ *   block_size, at most ctx_lens[b] and max_shared, the same for all rows of a
+ *   group, 0 for a row that shares nothing (such rows need no group; every row with
+ *   a prefix must be in one). The prefix is read through the block table of the
+ *   group's first row; all its rows' tables must name the same blocks there.
+ * max_shared: the longest shared prefix (0: nothing is shared, and the call is
+ *   ps_paged_decode_ordered). split_keys: keys per piece of the prefix pass (a
+ *   multiple of 128; 0 = one piece), so that few groups fill the GPU.
+ * split_tokens cuts the keys behind the prefixes; seq_order orders sequences by them.
+ * workspace: ps_paged_decode_shared_workspace_bytes(...) bytes, 256-byte aligned, one
+ *   call at a time.
+ * Errors: a shared length that breaks these rules sets PS_DEVERR_LENGTH (the outputs
+ * of the rows concerned are then unspecified). Keys at or past ctx_lens[b] are not
+ * used, whatever their rows hold.
+ */
+PS_API int ps_paged_decode_shared(void* out, int64_t out_seq_stride, const void* query,
+                                  int64_t query_seq_stride, const void* k_pool,
+                                  const void* v_pool, int64_t num_blocks,
+                                  const int32_t* block_tables, int64_t block_table_stride,
+                                  const int32_t* ctx_lens, int num_seqs,
+                                  const int32_t* group_starts, int num_groups,
+                                  const int32_t* shared_lens, int max_group, int max_shared,
+                                  int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                  int max_blocks_per_seq, float scale, int split_keys,
+                                  int split_tokens, void* workspace, int64_t workspace_bytes,
+                                  int dtype, const int32_t* seq_order, int32_t* device_error,
+                                  void* stream);
+
+/* Bytes of workspace ps_paged_decode_shared needs for these sizes (0 for invalid ones). */
+PS_API int64_t ps_paged_decode_shared_workspace_bytes(int num_seqs, int num_q_heads, int head_dim,
+                                                      int block_size, int max_blocks_per_seq,
+                                                      int max_shared, int split_keys,
+                                                      int split_tokens);
+
+/*
  * ---- 8-bit KV cache ----
  *
  * The pools hold one code per value, in the layout of the 16-bit pools

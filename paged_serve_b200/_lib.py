@@ -88,6 +88,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _l, _p, _l, _p, _p, _l, _p, _l, _p, _i, _i, _i, _i, _i, _i, c_float, _i, _i, _p,
          _p],
     ),
+    "ps_paged_decode_shared": (
+        c_int,
+        [_p, _l, _p, _l, _p, _p, _l, _p, _l, _p, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i,
+         c_float, _i, _i, _p, _l, _i, _p, _p, _p],
+    ),
+    "ps_paged_decode_shared_workspace_bytes": (c_int64, [_i, _i, _i, _i, _i, _i, _i, _i]),
     "ps_cache_append_quant": (
         c_int, [_p, _p, _p, _p, _p, _p, _p, _l, _l, _l, _i, _i, _i, _l, _i, _i, _p, _p],
     ),

@@ -59,7 +59,27 @@ struct DecodeParams {
   int64_t new_v_stride;
   const int64_t* new_slots;
   int64_t num_slots;
+  // Optional shared prefix (ps_paged_decode_shared): the first shared_lens[b] keys of
+  // sequence b are attended by the prefix pass, which leaves pieces of pre_keys keys
+  // as unnormalised outputs pre_o and (running max, sum) pre_ml, rows
+  // (piece * num_seqs + b) * num_q_heads + head. Partitions cut the keys behind them.
+  const int32_t* shared_lens;
+  const float* pre_o;
+  const float2* pre_ml;
+  int pre_keys;
+  int pre_max;  // largest prefix the pieces hold
 };
+
+// Shared-prefix tokens of sequence b with ctx keys; 0 (and an error bit) when
+// the prefix is not whole blocks of the sequence or longer than the pieces hold.
+__device__ __forceinline__ int shared_prefix(const DecodeParams& p, int b, int ctx, bool report) {
+  const int pre = p.shared_lens[b];
+  if (pre < 0 || pre > ctx || pre > p.pre_max || pre % p.block_size != 0) {
+    if (report) set_device_error(p.err, PS_DEVERR_LENGTH);
+    return 0;
+  }
+  return pre;
+}
 
 // Sequence at position i of the launch order; -1 (and an error bit) for an
 // entry that is not a sequence index.
@@ -78,6 +98,7 @@ __device__ __forceinline__ int ordered_seq(const DecodeParams& p, int i) {
 // a sequence with ctx keys has ceil(ctx / part) partitions, and one unit even
 // without keys (its output is written as zeros). One CTA of 1024 threads; a
 // running block-wide prefix sum places each sequence's units.
+template <bool kShared>
 __global__ void __launch_bounds__(1024) decode_plan_kernel(const DecodeParams p) {
   pdl_trigger();
   pdl_wait();
@@ -94,6 +115,7 @@ __global__ void __launch_bounds__(1024) decode_plan_kernel(const DecodeParams p)
     if (b >= 0) {
       int ctx = p.ctx_lens[b];
       if (ctx > p.max_blocks * p.block_size) ctx = 0;  // the decode kernel reports it
+      if constexpr (kShared) ctx -= shared_prefix(p, b, ctx, false);
       ns = ctx <= 0 ? 1 : (ctx + p.part_tokens - 1) / p.part_tokens;
     }
     int x = ns;  // inclusive scan within the warp
@@ -129,7 +151,8 @@ __global__ void __launch_bounds__(1024) decode_plan_kernel(const DecodeParams p)
 
 // Merge the partitions of each split sequence: out = sum_s w_s O_s, with
 // w_s = 2^(lse_s - max lse) / sum. One warp per (sequence, query head).
-template <typename T, int D>
+// kShared: the pieces of the sequence's shared prefix are merged too.
+template <typename T, int D, bool kShared = false>
 __global__ void __launch_bounds__(128) decode_combine_kernel(const DecodeParams p) {
   pdl_trigger();
   pdl_wait();
@@ -144,12 +167,19 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const DecodeParams 
   const int qh = warp_global % p.num_q_heads;
   int ctx = p.ctx_lens[b];
   if (ctx > p.max_blocks * p.block_size) ctx = 0;
+  int pre = 0;
+  if constexpr (kShared) pre = shared_prefix(p, b, ctx, false);
+  ctx -= pre;
   const int nsplit = (ctx + p.part_tokens - 1) / p.part_tokens;
   if (nsplit <= 1) return;
   const int64_t base = static_cast<int64_t>(b) * p.max_splits * p.num_q_heads + qh;
   float mmax = -INFINITY;
   for (int s = lane; s < nsplit; s += 32)
     mmax = fmaxf(mmax, p.ws_lse[base + static_cast<int64_t>(s) * p.num_q_heads]);
+  const int npre = kShared && pre > 0 ? (pre + p.pre_keys - 1) / p.pre_keys : 0;
+  const int64_t pre_row = static_cast<int64_t>(b) * p.num_q_heads + qh;
+  const int64_t pre_step = static_cast<int64_t>(p.num_seqs) * p.num_q_heads;
+  for (int s = lane; s < npre; s += 32) mmax = fmaxf(mmax, p.pre_ml[pre_row + s * pre_step].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mmax = fmaxf(mmax, __shfl_xor_sync(0xffffffffu, mmax, o));
   constexpr int kPer = D / 32;  // dims per lane
@@ -198,6 +228,13 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const DecodeParams 
       for (int u = 0; u < 4; ++u) add(__shfl_sync(0xffffffffu, wl, k + u), v[u]);
     }
     for (; k < n; ++k) add(__shfl_sync(0xffffffffu, wl, k), load(s0 + k));
+  }
+  for (int s = 0; s < npre; ++s) {
+    const int64_t row = pre_row + s * pre_step;
+    const float2 ml = p.pre_ml[row];
+    const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mmax);
+    wsum += w * (ml.y - 1.f);  // add() counts the weight once
+    add(w, *reinterpret_cast<const Vec*>(p.pre_o + row * D + lane * kPer));
   }
   const float inv = (wsum > 0.f) ? 1.f / wsum : 0.f;
   T* orow = static_cast<T*>(p.out) + b * p.out_stride + static_cast<int64_t>(qh) * D + lane * kPer;

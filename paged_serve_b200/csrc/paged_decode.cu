@@ -22,6 +22,7 @@
 #include <cudaTypedefs.h>
 
 #include "decode_common.cuh"
+#include "shared_prefix.h"
 
 namespace ps {
 namespace {
@@ -58,7 +59,10 @@ struct DecodeSmem {
 // kList: persistent CTAs (one per resident slot) claim (kv head, unit) pairs of
 // the split-K work list from an atomic counter, one ahead; otherwise one CTA
 // per (kv head, 1, sequence).
-template <typename T, int D, int NW, int NS, int BS, int R, bool kList>
+// kShared: a sequence's first shared_lens[b] keys belong to the prefix pass (the
+// kernel launched just before this one); this kernel walks the keys behind them
+// without waiting for that pass, and merges its pieces at the end.
+template <typename T, int D, int NW, int NS, int BS, int R, bool kList, bool kShared = false>
 __global__ void __launch_bounds__(NW * 32)
     paged_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap) {
@@ -89,7 +93,7 @@ __global__ void __launch_bounds__(NW * 32)
     for (int i = 0; i < NW * NS; ++i) mbar_init(&bars[i], 1);
     fence_barrier_init();
   }
-  pdl_wait();
+  if constexpr (!kShared) pdl_wait();
 
   // Work units: one (sequence, partition) per CTA, or, for split-K, (kv head,
   // planned unit) pairs claimed one at a time (thread 0 claims the next while
@@ -138,6 +142,12 @@ __global__ void __launch_bounds__(NW * 32)
     if (threadIdx.x == 0 && split == 0) set_device_error(p.err, PS_DEVERR_LENGTH);
     ctx = 0;
   }
+  const bool any_keys = ctx > 0;
+  int pre = 0;
+  if constexpr (kShared) {
+    if (any_keys) pre = shared_prefix(p, b, ctx, threadIdx.x == 0);
+    ctx -= pre;  // from here on: the sequence's own keys, behind the prefix
+  }
   const int nsplit = (ctx + p.part_tokens - 1) / p.part_tokens;
   // Fused append: this (sequence, kv head)'s new K/V row goes to its slot, in
   // the last partition, which only this unit reads. Thread t < 2*D/8 moves 16 B.
@@ -161,7 +171,8 @@ __global__ void __launch_bounds__(NW * 32)
     *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
     return true;
   };
-  if (ctx <= 0) {
+  if (!any_keys) {
+    if constexpr (kShared) pdl_wait();
     if (writer) write_row(threadIdx.x);  // nothing of this launch reads it
     // No keys: the output is defined as zeros (nothing to attend to).
     if (split == 0) {
@@ -170,7 +181,7 @@ __global__ void __launch_bounds__(NW * 32)
     }
     continue;
   }
-  if (split >= nsplit) continue;
+  if (split >= max(nsplit, kShared ? 1 : 0)) continue;
 
   const int t_begin = split * p.part_tokens;
   const int t_end = min(ctx, t_begin + p.part_tokens);
@@ -180,7 +191,7 @@ __global__ void __launch_bounds__(NW * 32)
   const int nblk = (t_end - t_begin + BS - 1) / BS;
 
   // Stage this partition's block ids, validated, in shared memory.
-  const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride + blk_begin;
+  const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride + blk_begin + pre / BS;
   for (int i = threadIdx.x; i < nblk; i += blockDim.x) {
     int32_t id = bt[i];
     if (id < 0 || id >= p.num_blocks) {
@@ -334,10 +345,25 @@ __global__ void __launch_bounds__(NW * 32)
     }
 
     // ---- O += P V
+    // kShared: values of keys past the end become 0, whatever their rows hold (this
+    // lane's keys are 2 q4, 2 q4 + 1 in the low and high half of b00/b10, and the
+    // same plus 8 in b01/b11).
+    uint32_t live0 = 0xffffffffu, live1 = 0xffffffffu;
+    if constexpr (kShared) {
+      const int k0 = t_end - tok0 - 2 * q4;
+      live0 = k0 >= 2 ? 0xffffffffu : k0 == 1 ? 0x0000ffffu : 0u;
+      live1 = k0 >= 10 ? 0xffffffffu : k0 == 9 ? 0x0000ffffu : 0u;
+    }
 #pragma unroll
     for (int jj = 0; jj < kNTiles / 2; ++jj) {
       uint32_t b00, b01, b10, b11;
       ldsm_x4_t(vbase + G::off(pv_t, 2 * jj + pv_c), b00, b01, b10, b11);
+      if constexpr (kShared) {
+        b00 &= live0;
+        b01 &= live1;
+        b10 &= live0;
+        b11 &= live1;
+      }
       Mma<T>::run(o[2 * jj], pa0, pa1, pa2, pa3, b00, b01);
       Mma<T>::run(o[2 * jj + 1], pa0, pa1, pa2, pa3, b10, b11);
     }
@@ -394,13 +420,22 @@ __global__ void __launch_bounds__(NW * 32)
   }
   __syncthreads();
 
-  const bool single = (nsplit == 1);
+  const bool single = kShared ? nsplit <= 1 : nsplit == 1;
+  // The prefix pass has left its pieces (and whatever runs after this kernel waits
+  // for that pass too, since every CTA does).
+  if constexpr (kShared) pdl_wait();
+  const int npre = kShared && single && pre > 0 ? (pre + p.pre_keys - 1) / p.pre_keys : 0;
   for (int idx = threadIdx.x; idx < group * (D / 4); idx += blockDim.x) {
     const int g = idx / (D / 4);
     const int d = (idx % (D / 4)) * 4;
     float mmax = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) mmax = fmaxf(mmax, ms[w * R + g]);
+    const int64_t pre_row = static_cast<int64_t>(b) * p.num_q_heads + h * group + g;
+    const int64_t pre_step = static_cast<int64_t>(p.num_seqs) * p.num_q_heads;
+    if constexpr (kShared) {
+      for (int s = 0; s < npre; ++s) mmax = fmaxf(mmax, p.pre_ml[pre_row + s * pre_step].x);
+    }
     float lsum = 0.f;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -413,6 +448,20 @@ __global__ void __launch_bounds__(NW * 32)
       acc[1] += ov.y * sc;
       acc[2] += ov.z * sc;
       acc[3] += ov.w * sc;
+    }
+    if constexpr (kShared) {
+#pragma unroll 4
+      for (int s = 0; s < npre; ++s) {
+        const int64_t row = pre_row + s * pre_step;
+        const float2 ml = p.pre_ml[row];
+        const float sc = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mmax);
+        const float4 ov = *reinterpret_cast<const float4*>(p.pre_o + row * D + d);
+        lsum += ml.y * sc;
+        acc[0] += ov.x * sc;
+        acc[1] += ov.y * sc;
+        acc[2] += ov.z * sc;
+        acc[3] += ov.w * sc;
+      }
     }
     const float inv = (lsum > 0.f) ? 1.f / lsum : 0.f;
     const int qh = h * group + g;
@@ -438,6 +487,7 @@ __global__ void __launch_bounds__(NW * 32)
     __syncthreads();
   }
   }  // work units
+  if constexpr (kShared) pdl_wait();  // also in CTAs that had no unit
 }
 
 // Longest-first order of the sequences for a decode launch: a counting sort of
@@ -514,19 +564,23 @@ constexpr int kNS = 2;  // TMA stages per warp
 template <int D>
 constexpr int unsplit_warps() { return D == 64 ? 8 : kNW; }
 
-template <typename T, int D, int BS, int R>
+template <typename T, int D, int BS, int R, bool kShared>
 int launch_decode(const DecodeParams& p, const CUtensorMap& km, const CUtensorMap& vm,
-                  cudaStream_t s) {
+                  cudaStream_t s, const SharedPrefix* prefix) {
   using SM = DecodeSmem<D, kNW, kNS>;
   const size_t smem = SM::bytes(p.table_cap);
   if (p.max_splits <= 1) {
     constexpr int NWU = unsplit_warps<D>();
-    auto kern = paged_decode_kernel<T, D, NWU, kNS, BS, R, false>;
+    auto kern = paged_decode_kernel<T, D, NWU, kNS, BS, R, false, kShared>;
     static size_t configured[64] = {};
     const size_t smem_u = DecodeSmem<D, NWU, kNS>::bytes(p.table_cap);
     int st = reserve_smem(kern, smem_u, configured);
     if (st != PS_OK) return st;
     dim3 grid(p.num_kv_heads, 1, p.num_launch);
+    if constexpr (kShared) {
+      st = launch_shared_prefix(*prefix, s);
+      if (st != PS_OK) return st;
+    }
     const cudaError_t e = launch_pdl(kern, grid, dim3(NWU * 32), smem_u, s, p, km, vm);
     if (e != cudaSuccess)
       return fail(PS_ERR_CUDA, "ps_paged_decode: launch failed: %s", cudaGetErrorString(e));
@@ -535,7 +589,7 @@ int launch_decode(const DecodeParams& p, const CUtensorMap& km, const CUtensorMa
   // Split-K: plan the (sequence, partition) units on the device, then one
   // persistent CTA per resident slot claims them; the grid does not depend on
   // the lengths, so the launch sequence can be captured in a CUDA graph.
-  auto kern = paged_decode_kernel<T, D, kNW, kNS, BS, R, true>;
+  auto kern = paged_decode_kernel<T, D, kNW, kNS, BS, R, true, kShared>;
   static size_t configured[64] = {};
   int st = reserve_smem(kern, smem, configured);
   if (st != PS_OK) return st;
@@ -559,43 +613,50 @@ int launch_decode(const DecodeParams& p, const CUtensorMap& km, const CUtensorMa
   lock.unlock();
   cudaError_t e = cudaSuccess;
   if (!p.planned) {
-    e = launch_pdl(decode_plan_kernel, dim3(1), dim3(1024), 0, s, p);
+    e = launch_pdl(decode_plan_kernel<kShared>, dim3(1), dim3(1024), 0, s, p);
     if (e != cudaSuccess)
       return fail(PS_ERR_CUDA, "ps_paged_decode(plan): launch failed: %s", cudaGetErrorString(e));
+  }
+  if constexpr (kShared) {
+    st = launch_shared_prefix(*prefix, s);
+    if (st != PS_OK) return st;
   }
   e = launch_pdl(kern, dim3(per_sm * sms), dim3(kNW * 32), smem, s, p, km, vm);
   if (e != cudaSuccess)
     return fail(PS_ERR_CUDA, "ps_paged_decode: launch failed: %s", cudaGetErrorString(e));
   const int warps = p.num_launch * p.num_q_heads;
-  e = launch_pdl(decode_combine_kernel<T, D>, dim3((warps + 3) / 4), dim3(128), 0, s, p);
+  e = launch_pdl(decode_combine_kernel<T, D, kShared>, dim3((warps + 3) / 4), dim3(128), 0, s, p);
   if (e != cudaSuccess)
     return fail(PS_ERR_CUDA, "ps_paged_decode(combine): launch failed: %s",
                 cudaGetErrorString(e));
   return check_launch("ps_paged_decode(combine)");
 }
 
-template <typename T, int D, int R>
+template <typename T, int D, int R, bool kShared>
 int dispatch_bs(const DecodeParams& p, const CUtensorMap& km, const CUtensorMap& vm,
-                cudaStream_t s, int block_size) {
-  if (block_size == 8) return launch_decode<T, D, 8, R>(p, km, vm, s);
-  if (block_size == 32) return launch_decode<T, D, 32, R>(p, km, vm, s);
-  return launch_decode<T, D, 16, R>(p, km, vm, s);
+                cudaStream_t s, int block_size, const SharedPrefix* prefix) {
+  if (block_size == 8) return launch_decode<T, D, 8, R, kShared>(p, km, vm, s, prefix);
+  if (block_size == 32) return launch_decode<T, D, 32, R, kShared>(p, km, vm, s, prefix);
+  return launch_decode<T, D, 16, R, kShared>(p, km, vm, s, prefix);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kShared>
 int dispatch_rows(const DecodeParams& p, const CUtensorMap& km, const CUtensorMap& vm,
-                  cudaStream_t s, int block_size) {
-  return p.group > 8 ? dispatch_bs<T, D, 16>(p, km, vm, s, block_size)
-                     : dispatch_bs<T, D, 8>(p, km, vm, s, block_size);
+                  cudaStream_t s, int block_size, const SharedPrefix* prefix) {
+  return p.group > 8 ? dispatch_bs<T, D, 16, kShared>(p, km, vm, s, block_size, prefix)
+                     : dispatch_bs<T, D, 8, kShared>(p, km, vm, s, block_size, prefix);
 }
 
+template <bool kShared>
 int dispatch_decode(const DecodeParams& p, const CUtensorMap& km, const CUtensorMap& vm,
-                    cudaStream_t s, int dtype, int head_dim, int block_size) {
+                    cudaStream_t s, int dtype, int head_dim, int block_size,
+                    const SharedPrefix* prefix = nullptr) {
   if (dtype == PS_DTYPE_BF16)
-    return head_dim == 128 ? dispatch_rows<__nv_bfloat16, 128>(p, km, vm, s, block_size)
-                           : dispatch_rows<__nv_bfloat16, 64>(p, km, vm, s, block_size);
-  return head_dim == 128 ? dispatch_rows<__half, 128>(p, km, vm, s, block_size)
-                         : dispatch_rows<__half, 64>(p, km, vm, s, block_size);
+    return head_dim == 128
+               ? dispatch_rows<__nv_bfloat16, 128, kShared>(p, km, vm, s, block_size, prefix)
+               : dispatch_rows<__nv_bfloat16, 64, kShared>(p, km, vm, s, block_size, prefix);
+  return head_dim == 128 ? dispatch_rows<__half, 128, kShared>(p, km, vm, s, block_size, prefix)
+                         : dispatch_rows<__half, 64, kShared>(p, km, vm, s, block_size, prefix);
 }
 
 }  // namespace
@@ -664,7 +725,8 @@ int decode_entry(const char* fn, void* out, int64_t out_seq_stride, const void* 
                  int head_dim, int block_size, int max_blocks_per_seq, float scale,
                  int split_tokens, void* workspace, int64_t workspace_bytes, int dtype,
                  const int32_t* seq_order, const NewToken* nt, int32_t* device_error,
-                 void* stream, int num_launch = -1, bool planned = false) {
+                 void* stream, int num_launch = -1, bool planned = false,
+                 const SharedPrefix* shared = nullptr) {
   int part = 0, max_splits = 0, table_cap = 0;
   int vst = validate_decode(fn, out, out_seq_stride, query, query_seq_stride, k_pool, v_pool,
                             num_blocks, block_tables, block_table_stride, ctx_lens, num_seqs,
@@ -735,7 +797,15 @@ int decode_entry(const char* fn, void* out, int64_t out_seq_stride, const void* 
   if (st != PS_OK) return st;
 
   cudaStream_t s = as_stream(stream);
-  return dispatch_decode(p, km, vm, s, dtype, head_dim, block_size);
+  if (shared) {
+    p.shared_lens = shared->shared_lens;
+    p.pre_o = shared->part_o;
+    p.pre_ml = shared->part_ml;
+    p.pre_keys = shared->piece_keys;
+    p.pre_max = shared->pieces * shared->piece_keys;
+    return dispatch_decode<true>(p, km, vm, s, dtype, head_dim, block_size, shared);
+  }
+  return dispatch_decode<false>(p, km, vm, s, dtype, head_dim, block_size);
 }
 }  // namespace
 
@@ -845,7 +915,7 @@ extern "C" int ps_paged_decode_plan(const int32_t* ctx_lens, int num_seqs,
   p.item_count = reinterpret_cast<int32_t*>(ws + o_bytes + lse_bytes + item_bytes);
   p.item_next = p.item_count + 1;
   const cudaError_t e =
-      launch_pdl(decode_plan_kernel, dim3(1), dim3(1024), 0, as_stream(stream), p);
+      launch_pdl(decode_plan_kernel<false>, dim3(1), dim3(1024), 0, as_stream(stream), p);
   if (e != cudaSuccess) return fail(PS_ERR_CUDA, "%s: launch failed: %s", fn, cudaGetErrorString(e));
   return check_launch(fn);
 }
@@ -866,6 +936,122 @@ extern "C" int ps_paged_decode_append_planned(
                       block_table_stride, ctx_lens, num_seqs, num_q_heads, num_kv_heads, head_dim,
                       block_size, max_blocks_per_seq, scale, split_tokens, workspace,
                       workspace_bytes, dtype, seq_order, &nt, device_error, stream, -1, true);
+}
+
+// ------------------------------------------------------------ shared prefixes
+namespace ps {
+namespace {
+// Pieces of the prefix pass and where a workspace holds their partials (outputs,
+// then running maxima and sums, then the split-K workspace of the own keys).
+struct SharedLayout {
+  int piece_keys = 0;
+  int pieces = 0;
+  int64_t o_bytes = 0;
+  int64_t ml_bytes = 0;
+};
+
+SharedLayout shared_layout(int num_seqs, int num_q_heads, int head_dim, int max_shared,
+                           int split_keys) {
+  SharedLayout l;
+  if (max_shared <= 0) return l;
+  l.piece_keys = split_keys > 0 ? split_keys : (max_shared + 127) / 128 * 128;
+  l.pieces = (max_shared + l.piece_keys - 1) / l.piece_keys;
+  const int64_t rows = static_cast<int64_t>(l.pieces) * num_seqs * num_q_heads;
+  l.o_bytes = (rows * head_dim * 4 + 255) / 256 * 256;
+  l.ml_bytes = (rows * 8 + 255) / 256 * 256;
+  return l;
+}
+}  // namespace
+}  // namespace ps
+
+extern "C" int64_t ps_paged_decode_shared_workspace_bytes(int num_seqs, int num_q_heads,
+                                                          int head_dim, int block_size,
+                                                          int max_blocks_per_seq, int max_shared,
+                                                          int split_keys, int split_tokens) {
+  ps::NvtxRange nvtx_range("ps_paged_decode_shared_workspace_bytes");
+  if (num_seqs <= 0 || num_q_heads <= 0 || head_dim <= 0 || max_blocks_per_seq <= 0 ||
+      block_size <= 0 || max_shared < 0 || max_shared > (1 << 30) || split_keys < 0 ||
+      split_keys % 128)
+    return 0;
+  const SharedLayout l = shared_layout(num_seqs, num_q_heads, head_dim, max_shared, split_keys);
+  return l.o_bytes + l.ml_bytes +
+         ps_paged_decode_workspace_bytes(num_seqs, num_q_heads, head_dim, block_size,
+                                         max_blocks_per_seq, split_tokens);
+}
+
+extern "C" int ps_paged_decode_shared(
+    void* out, int64_t out_seq_stride, const void* query, int64_t query_seq_stride,
+    const void* k_pool, const void* v_pool, int64_t num_blocks, const int32_t* block_tables,
+    int64_t block_table_stride, const int32_t* ctx_lens, int num_seqs, const int32_t* group_starts,
+    int num_groups, const int32_t* shared_lens, int max_group, int max_shared, int num_q_heads,
+    int num_kv_heads, int head_dim, int block_size, int max_blocks_per_seq, float scale,
+    int split_keys, int split_tokens, void* workspace, int64_t workspace_bytes, int dtype,
+    const int32_t* seq_order, int32_t* device_error, void* stream) {
+  ps::NvtxRange nvtx_range("ps_paged_decode_shared");
+  const char* fn = "ps_paged_decode_shared";
+  int part = 0, max_splits = 0, table_cap = 0;
+  const int vst = validate_decode(fn, out, out_seq_stride, query, query_seq_stride, k_pool, v_pool,
+                                  num_blocks, block_tables, block_table_stride, ctx_lens, num_seqs,
+                                  num_q_heads, num_kv_heads, head_dim, block_size,
+                                  max_blocks_per_seq, split_tokens, dtype, &part, &max_splits,
+                                  &table_cap);
+  if (vst != PS_OK || num_seqs == 0) return vst;
+  if (max_shared < 0 || max_shared > static_cast<int64_t>(max_blocks_per_seq) * block_size)
+    return fail(PS_ERR_INVALID, "%s: max_shared %d outside [0, max_blocks_per_seq * block_size]",
+                fn, max_shared);
+  if (split_keys < 0 || split_keys % 128)
+    return fail(PS_ERR_INVALID, "%s: split_keys %d must be a non-negative multiple of 128", fn,
+                split_keys);
+  if (num_groups < 0 || num_groups > num_seqs || max_group < 0 || max_group > num_seqs)
+    return fail(PS_ERR_INVALID, "%s: num_groups %d and max_group %d must be in [0, num_seqs]", fn,
+                num_groups, max_group);
+  if (max_shared == 0 || num_groups == 0 || max_group == 0)  // nothing is shared
+    return decode_entry(fn, out, out_seq_stride, query, query_seq_stride, k_pool, v_pool,
+                        num_blocks, block_tables, block_table_stride, ctx_lens, num_seqs,
+                        num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, scale,
+                        split_tokens, workspace, workspace_bytes, dtype, seq_order, nullptr,
+                        device_error, stream);
+  if (!group_starts || !shared_lens)
+    return fail(PS_ERR_INVALID, "%s: null group_starts/shared_lens", fn);
+  const int64_t need = ps_paged_decode_shared_workspace_bytes(
+      num_seqs, num_q_heads, head_dim, block_size, max_blocks_per_seq, max_shared, split_keys,
+      split_tokens);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+    return fail(PS_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %lld bytes", fn,
+                (long long)need);
+  const SharedLayout l = shared_layout(num_seqs, num_q_heads, head_dim, max_shared, split_keys);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  SharedPrefix a{};
+  a.fn = fn;
+  a.query = query;
+  a.query_seq_stride = query_seq_stride;
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.num_blocks = num_blocks;
+  a.block_tables = block_tables;
+  a.block_table_stride = block_table_stride;
+  a.group_starts = group_starts;
+  a.shared_lens = shared_lens;
+  a.num_groups = num_groups;
+  a.max_group = max_group;
+  a.num_seqs = num_seqs;
+  a.num_q_heads = num_q_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.head_dim = head_dim;
+  a.block_size = block_size;
+  a.max_blocks = max_blocks_per_seq;
+  a.pieces = l.pieces;
+  a.piece_keys = l.piece_keys;
+  a.scale = scale;
+  a.part_o = reinterpret_cast<float*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + l.o_bytes);
+  a.dtype = dtype;
+  a.device_error = device_error;
+  return decode_entry(fn, out, out_seq_stride, query, query_seq_stride, k_pool, v_pool, num_blocks,
+                      block_tables, block_table_stride, ctx_lens, num_seqs, num_q_heads,
+                      num_kv_heads, head_dim, block_size, max_blocks_per_seq, scale, split_tokens,
+                      ws + l.o_bytes + l.ml_bytes, workspace_bytes - l.o_bytes - l.ml_bytes, dtype,
+                      seq_order, nullptr, device_error, stream, -1, false, &a);
 }
 
 // ------------------------------------------------------------ allocation-free variant

@@ -521,7 +521,7 @@ int launch_quant(const QuantDecodeParams& qp, const CUtensorMap& km, const CUten
   if (e != cudaSuccess || per_sm <= 0)
     return fail(PS_ERR_CUDA, "%s: occupancy query failed: %s", fn, cudaGetErrorString(e));
   if (!p.planned) {
-    e = launch_pdl(decode_plan_kernel, dim3(1), dim3(1024), 0, s, p);
+    e = launch_pdl(decode_plan_kernel<false>, dim3(1), dim3(1024), 0, s, p);
     if (e != cudaSuccess)
       return fail(PS_ERR_CUDA, "%s(plan): launch failed: %s", fn, cudaGetErrorString(e));
   }

@@ -43,6 +43,7 @@
 
 #include "capi_internal.h"
 #include "common.cuh"
+#include "shared_prefix.h"
 #include "tcgen05.cuh"
 
 namespace ps {
@@ -130,6 +131,9 @@ struct PrefillParams {
   int num_units;     // num_items * splits
   float* part_o;     // [num_units][2 tiles][128 rows][D] fp32
   float2* part_ml;   // [num_units][2 tiles][128 rows] (running max, log2 units; row sum)
+  // Shared-prefix pass of a decode step (kShared): a "sequence" is a group of
+  // neighbouring batch rows, q_starts their group starts [num_seqs + 1], ctx_lens the
+  // shared prefix of each batch row; partials are [splits][num_rows][Hq] rows.
   float scale_log2;
   int32_t* err;
 };
@@ -144,7 +148,7 @@ struct PrefillParams {
 // tiles.
 struct Item {
   int b, h, t0, q_len, ctx, q_start, ntiles, nblk_seq, last_key;
-  int unit, j0;  // the unit, and its first key tile (0 unless split)
+  int unit, j0;  // the unit (kShared: the piece), and its first key tile (0 unless split)
   bool partial;  // the item spans several pieces: write partials, not the output
 };
 
@@ -155,7 +159,10 @@ struct Item {
 // (their pieces, not their tiles, spread the work). The unsplit kernel is its
 // own instantiation, so none of the piece arithmetic reaches its loops
 // (measured 5% slower on the prefix workload when it did).
-template <bool kSplit>
+//
+// kShared (with kSplit): the keys of group w.b's shared prefix, which every one of
+// its rows attends whole; the prefix is read through the block table of its first row.
+template <bool kSplit, bool kShared = false>
 __device__ __forceinline__ bool decode_item(const PrefillParams& p, int u, Item& w, bool report) {
   int it = u, piece = 0;
   if constexpr (kSplit) {
@@ -168,8 +175,35 @@ __device__ __forceinline__ bool decode_item(const PrefillParams& p, int u, Item&
   const int qt = nq - 1 - (it % nq + wave) % nq;
   w.b = g / p.num_kv_heads;
   w.h = g % p.num_kv_heads;
-  w.q_len = p.q_lens[w.b];
   w.t0 = qt * 2 * p.tokens_per_tile;
+  if constexpr (kShared) {
+    static_assert(kSplit, "the shared-prefix pass writes partials");
+    w.q_start = p.q_starts[w.b];
+    w.q_len = p.q_starts[w.b + 1] - w.q_start;
+    if (w.t0 >= w.q_len) return false;
+    if (w.q_start < 0 || w.q_len > p.num_rows - w.q_start ||
+        w.q_len > nq * 2 * p.tokens_per_tile) {
+      if (report) set_device_error(p.err, PS_DEVERR_LENGTH);
+      return false;
+    }
+    w.ctx = p.ctx_lens[w.q_start];
+    w.last_key = w.ctx;
+    const int64_t room = static_cast<int64_t>(p.splits) * p.split_tiles * kN;  // pieces' keys
+    if (w.ctx <= 0 || w.ctx > p.max_blocks * p.block_size || w.ctx > room ||
+        w.ctx % p.block_size != 0) {
+      if (report && w.ctx != 0) set_device_error(p.err, PS_DEVERR_LENGTH);
+      return false;
+    }
+    const int item_tiles = (w.ctx + kN - 1) / kN;
+    w.unit = piece;
+    w.j0 = piece * p.split_tiles;
+    if (w.j0 >= item_tiles) return false;
+    w.ntiles = min(p.split_tiles, item_tiles - w.j0);
+    w.partial = true;
+    w.nblk_seq = w.ctx / p.block_size;
+    return true;
+  }
+  w.q_len = p.q_lens[w.b];
   if (w.t0 >= w.q_len) return false;
   w.ctx = p.ctx_lens[w.b];
   w.q_start = p.q_starts[w.b];
@@ -258,7 +292,7 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
 // Softmax + epilogue of one query tile; 128 threads, thread = TMEM lane = row.
 // g0: tiles this CTA processed before the item (S and P barrier phases);
 // n: items before it (O barrier phase). Returns false once aborted.
-template <typename T, int D, bool kSplit>
+template <typename T, int D, bool kSplit, bool kShared>
 __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* bars,
                                              volatile int* abort, uint32_t tmem, int tile, int r,
                                              int warp_in_tile, const Item& w, int g0, int n) {
@@ -270,8 +304,9 @@ __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* b
   const int tpt = p.tokens_per_tile;
   const int tok = r / G;
   const bool row_real = (r < G * tpt) && (t0_tile + tok < q_len);
-  const int limit = row_real ? ctx + t0_tile + tok : last_key - 1;  // last key this row sees
-  const int tile_min_limit = ctx + t0_tile;  // smallest limit among this tile's real rows
+  // Last key this row sees, and the smallest such key among this tile's real rows.
+  const int limit = row_real && !kShared ? ctx + t0_tile + tok : last_key - 1;
+  const int tile_min_limit = kShared ? last_key - 1 : ctx + t0_tile;
   const uint32_t lane_tmem = tmem + (static_cast<uint32_t>(warp_in_tile * 32) << 16);
   const uint32_t s_col = kTmemS + tile * kN;
   const uint32_t o_col = kTmemO + tile * D;
@@ -307,7 +342,10 @@ __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* b
 #pragma unroll
     for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[kN - 4 + e]);
     const float mt = max3f(mx[0], mx[1], fmaxf(mx[2], mx[3])) * p.scale_log2;
-    const bool rescale = __any_sync(0xffffffffu, mt > m_used + kRescaleThreshold);
+    // kShared: rows that hold no query (what shared memory held before, where 128 is
+    // no multiple of G) do not vote, so the bits of the real rows never depend on them.
+    const bool votes = !kShared || row_real;
+    const bool rescale = __any_sync(0xffffffffu, votes && mt > m_used + kRescaleThreshold);
     float alpha = 1.f;
     if (rescale) {
       const float m_new = fmaxf(m_used, mt);
@@ -378,7 +416,13 @@ __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* b
     for (int c = 0; c < D / 32; ++c) tmem_ld32(lane_tmem + o_col + c * 32, oall[c]);
     tmem_wait_ld();
     if (row_real) {
-      const int64_t prow = (static_cast<int64_t>(w.unit) * 2 + tile) * kM + r;
+      int64_t prow = (static_cast<int64_t>(w.unit) * 2 + tile) * kM + r;
+      if constexpr (kShared) {
+        const int row = q_start + t0_tile + tok;
+        prow = (static_cast<int64_t>(w.unit) * p.num_rows + row) * p.num_q_heads + h * G + r % G;
+        // A row that names another length would merge pieces it does not have.
+        if (p.ctx_lens[row] != ctx) set_device_error(p.err, PS_DEVERR_LENGTH);
+      }
       float4* po = reinterpret_cast<float4*>(p.part_o + prow * D);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
@@ -424,7 +468,7 @@ __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* b
 }
 
 // BS = tokens per KV block (8, 16 or 32): a 128-key tile is 128/BS block boxes.
-template <typename T, int D, int BS, bool kSplit>
+template <typename T, int D, int BS, bool kSplit, bool kShared>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap qmap,
                          const __grid_constant__ CUtensorMap kmap,
@@ -445,8 +489,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // Launched with programmatic stream serialization: barrier set-up and the
   // TMEM allocation overlap the previous kernel's end; global memory is
-  // touched only after pdl_wait().
-  pdl_trigger();
+  // touched only after pdl_wait(). The shared-prefix pass triggers only then: the
+  // decode over the sequences' own keys that follows it reads the caller's data
+  // without waiting for this kernel, so what came before must be complete.
+  if constexpr (!kShared) pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kNumBars; ++i) mbar_init(&bars[i], (i >= C::kBarP && i < C::kBarP + 2) ? 128 : 1);
     *abort = 0;
@@ -458,6 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = misc[0];
   pdl_wait();
+  if constexpr (kShared) pdl_trigger();
 
   // Persistent: CTA c takes items c, c + gridDim.x, ... Every role walks the
   // same items; ring positions and barrier phases carry over from item to item.
@@ -480,8 +527,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int it = blockIdx.x; ok && it < p.num_units; it += gridDim.x) {
       Item w;
-      if (!decode_item<kSplit>(p, it, w, lane == 0)) continue;
-      const int32_t* bt = p.block_tables + static_cast<int64_t>(w.b) * p.bt_stride;
+      if (!decode_item<kSplit, kShared>(p, it, w, lane == 0)) continue;
+      const int32_t* bt = p.block_tables + static_cast<int64_t>(kShared ? w.q_start : w.b) * p.bt_stride;
       int window = -32;  // first block index held by the lanes' `my_row`
       int32_t my_row = 0;
       // Block-row coordinates of key tile j (uniform across the warp).
@@ -625,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int it = blockIdx.x; ok && it < p.num_units; it += gridDim.x) {
       Item w;
-      if (!decode_item<kSplit>(p, it, w, false)) continue;
+      if (!decode_item<kSplit, kShared>(p, it, w, false)) continue;
       if (!(ok = wait_all(&bars[C::kBarQ], n & 1))) break;
       if (!(ok = wait_all(&bars[C::kBarKFull + kc % C::kKStages], (kc / C::kKStages) & 1))) break;
       tc_fence_after();
@@ -669,8 +716,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int g = 0, n = 0;
     for (int it = blockIdx.x; it < p.num_units; it += gridDim.x) {
       Item w;
-      if (!decode_item<kSplit>(p, it, w, false)) continue;
-      if (!softmax_tile<T, D, kSplit>(p, bars, abort, tmem, x, threadIdx.x & 127, warp & 3, w, g, n))
+      if (!decode_item<kSplit, kShared>(p, it, w, false)) continue;
+      if (!softmax_tile<T, D, kSplit, kShared>(p, bars, abort, tmem, x, threadIdx.x & 127, warp & 3, w, g, n))
         break;
       g += w.ntiles;
       ++n;
@@ -745,7 +792,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
 }
 
 // One per element type: the dynamic shared-memory opt-in is per kernel and per device.
-template <typename T, int D, int BS, bool kSplit>
+template <typename T, int D, int BS, bool kSplit, bool kShared = false>
 int launch_prefill(const PrefillParams& p, const CUtensorMap& qm, const CUtensorMap& km,
                    const CUtensorMap& vm, dim3 grid, cudaStream_t s) {
   static bool configured[64] = {};
@@ -757,7 +804,7 @@ int launch_prefill(const PrefillParams& p, const CUtensorMap& qm, const CUtensor
     // setmaxnreg.inc waits until the pool holds the registers it asks for: a
     // split above the launch allocation would never proceed, so refuse it here.
     cudaFuncAttributes fa{};
-    cudaError_t e = cudaFuncGetAttributes(&fa, paged_prefill_kernel<T, D, BS, kSplit>);
+    cudaError_t e = cudaFuncGetAttributes(&fa, paged_prefill_kernel<T, D, BS, kSplit, kShared>);
     if (e != cudaSuccess)
       return fail(PS_ERR_CUDA, "ps_paged_prefill: cannot read kernel attributes: %s",
                   cudaGetErrorString(e));
@@ -766,7 +813,7 @@ int launch_prefill(const PrefillParams& p, const CUtensorMap& qm, const CUtensor
                   "ps_paged_prefill: kernel built with %d registers x %d threads, the register "
                   "split needs %d",
                   fa.numRegs, kThreads, kRegPoolNeeded);
-    e = cudaFuncSetAttribute(paged_prefill_kernel<T, D, BS, kSplit>,
+    e = cudaFuncSetAttribute(paged_prefill_kernel<T, D, BS, kSplit, kShared>,
                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(Cfg<D>::kSmemBytes));
     if (e != cudaSuccess)
@@ -775,11 +822,11 @@ int launch_prefill(const PrefillParams& p, const CUtensorMap& qm, const CUtensor
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   lock.unlock();
-  cudaError_t e = launch_pdl(paged_prefill_kernel<T, D, BS, kSplit>, grid, dim3(kThreads),
+  cudaError_t e = launch_pdl(paged_prefill_kernel<T, D, BS, kSplit, kShared>, grid, dim3(kThreads),
                              Cfg<D>::kSmemBytes, s, p, qm, km, vm);
   if (e != cudaSuccess)
     return fail(PS_ERR_CUDA, "ps_paged_prefill: launch failed: %s", cudaGetErrorString(e));
-  if (kSplit) {
+  if constexpr (kSplit && !kShared) {
     const int64_t warps = static_cast<int64_t>(p.num_items) * 2 * kM;
     const dim3 cgrid(static_cast<unsigned>((warps + kCombineWarps - 1) / kCombineWarps));
     e = launch_pdl(prefill_combine_kernel<T, D>, cgrid, dim3(kCombineWarps * 32), 0, s, p);
@@ -788,6 +835,14 @@ int launch_prefill(const PrefillParams& p, const CUtensorMap& qm, const CUtensor
                   cudaGetErrorString(e));
   }
   return check_launch("ps_paged_prefill");
+}
+
+template <typename T, int D>
+int dispatch_shared(const PrefillParams& p, const CUtensorMap& qm, const CUtensorMap& km,
+                    const CUtensorMap& vm, dim3 grid, cudaStream_t s, int block_size) {
+  if (block_size == 8) return launch_prefill<T, D, 8, true, true>(p, qm, km, vm, grid, s);
+  if (block_size == 32) return launch_prefill<T, D, 32, true, true>(p, qm, km, vm, grid, s);
+  return launch_prefill<T, D, 16, true, true>(p, qm, km, vm, grid, s);
 }
 
 template <typename T, int D>
@@ -961,6 +1016,63 @@ int prefill_entry(const char* fn, void* out, int64_t out_token_stride, const voi
 }
 
 }  // namespace
+
+int launch_shared_prefix(const SharedPrefix& a, cudaStream_t s) {
+  const int group = a.num_q_heads / a.num_kv_heads;
+  const int tpt = kM / group;
+  PrefillParams p{};
+  p.block_tables = a.block_tables;
+  p.bt_stride = a.block_table_stride;
+  p.q_starts = a.group_starts;
+  p.ctx_lens = a.shared_lens;
+  p.num_blocks = a.num_blocks;
+  p.num_rows = a.num_seqs;
+  p.num_kv_heads = a.num_kv_heads;
+  p.num_q_heads = a.num_q_heads;
+  p.group = group;
+  p.tokens_per_tile = tpt;
+  p.max_blocks = a.max_blocks;
+  p.block_size = a.block_size;
+  p.num_seqs = a.num_groups;
+  p.num_q_tiles = (a.max_group + 2 * tpt - 1) / (2 * tpt);
+  const int64_t items = static_cast<int64_t>(p.num_q_tiles) * a.num_kv_heads * a.num_groups;
+  if (items * a.pieces >= (int64_t(1) << 31))
+    return fail(PS_ERR_INVALID, "%s: too many query tiles for one launch", a.fn);
+  p.num_items = static_cast<int>(items);
+  p.splits = a.pieces;
+  p.split_tiles = a.piece_keys / kN;
+  p.num_units = static_cast<int>(items * a.pieces);
+  p.part_o = a.part_o;
+  p.part_ml = a.part_ml;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.err = a.device_error;
+
+  CUtensorMap qm, km, vm;
+  const uint64_t dims[3] = {static_cast<uint64_t>(a.head_dim), static_cast<uint64_t>(a.num_q_heads),
+                            static_cast<uint64_t>(a.num_seqs)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(a.head_dim) * 2,
+                               static_cast<uint64_t>(a.query_seq_stride) * 2};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(group), static_cast<uint32_t>(tpt)};
+  int st = encode_tmap_16bit(&qm, const_cast<void*>(a.query), 3, dims, strides, box,
+                             CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st != PS_OK) return st;
+  const uint64_t rows = static_cast<uint64_t>(a.num_blocks) * a.num_kv_heads * a.block_size;
+  st = get_pool_tmap(a.k_pool, rows, a.head_dim, a.block_size, &km);
+  if (st != PS_OK) return st;
+  st = get_pool_tmap(a.v_pool, rows, a.head_dim, a.block_size, &vm);
+  if (st != PS_OK) return st;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess)
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const dim3 grid(static_cast<unsigned>(std::min(p.num_units, sms)));
+  if (a.dtype == PS_DTYPE_BF16)
+    return a.head_dim == 64
+               ? dispatch_shared<__nv_bfloat16, 64>(p, qm, km, vm, grid, s, a.block_size)
+               : dispatch_shared<__nv_bfloat16, 128>(p, qm, km, vm, grid, s, a.block_size);
+  return a.head_dim == 64 ? dispatch_shared<__half, 64>(p, qm, km, vm, grid, s, a.block_size)
+                          : dispatch_shared<__half, 128>(p, qm, km, vm, grid, s, a.block_size);
+}
+
 }  // namespace ps
 
 using namespace ps;

@@ -31,6 +31,7 @@ __all__ = [
     "paged_decode",
     "paged_decode_listed",
     "paged_decode_quant",
+    "paged_decode_shared",
     "paged_prefill",
     "stream_read",
     "swap_blocks",
@@ -692,6 +693,85 @@ def paged_decode_quant(
             _dtype_code(query), code, _err_ptr(device_error), _stream(a.dev),
         )
     _lib.check(st, "paged_decode_quant")
+    return a.out
+
+
+def decode_shared_workspace_bytes(
+    num_seqs: int, num_q_heads: int, head_dim: int, block_size: int, max_blocks_per_seq: int,
+    max_shared: int, split_keys: int, split_tokens: int,
+) -> int:
+    """Bytes of workspace :func:`paged_decode_shared` needs (0 if nothing is shared or split)."""
+    return int(_lib.load().ps_paged_decode_shared_workspace_bytes(
+        num_seqs, num_q_heads, head_dim, block_size, max_blocks_per_seq, max_shared, split_keys,
+        split_tokens))
+
+
+def shared_split_keys(group_sizes: list[int], num_q_heads: int, num_kv_heads: int,
+                      max_shared: int, num_sms: int) -> int:
+    """Keys per piece of a shared-prefix pass over groups of these sizes; 0 = one piece.
+
+    The pass has the prefill kernel's work items (pairs of 128-row query tiles, a row
+    being one sequence and query head of a KV head's group), so this is
+    :func:`prefill_split_keys` of their number.
+    """
+    pair = 2 * (128 // (num_q_heads // num_kv_heads))
+    items = sum(-(-n // pair) for n in group_sizes) * num_kv_heads
+    return prefill_split_keys(items, max_shared, num_sms)
+
+
+def paged_decode_shared(
+    query: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    group_starts: torch.Tensor,
+    shared_lens: torch.Tensor,
+    max_group: int,
+    max_shared: int,
+    scale: float,
+    split_keys: int = 0,
+    split_tokens: int = 0,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+    device_error: torch.Tensor | None = None,
+    seq_order: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`paged_decode` where neighbouring sequences share their leading blocks.
+
+    Group g is rows ``[group_starts[g], group_starts[g + 1])`` of the batch (int32
+    ``[groups + 1]``, at most ``max_group`` rows each); ``shared_lens`` (int32 [B]) gives
+    each row's shared keys: whole blocks, the same for all rows of a group, at most
+    ``max_shared``, 0 for rows that share nothing. A group's prefix is read once for all
+    its rows, in pieces of ``split_keys`` keys (:func:`shared_split_keys`; 0 = one
+    piece); the keys behind it go as in :func:`paged_decode`, cut by ``split_tokens``
+    and taken in ``seq_order`` (:func:`decode_order` of ``ctx_lens - shared_lens``).
+    ``workspace``: uint8, :func:`decode_shared_workspace_bytes`, allocated here when not
+    given. Keys past a sequence's length are ignored whatever their rows hold.
+    """
+    a = _DecodeArgs(query, k_pool, v_pool, block_tables, ctx_lens, out, workspace, device_error,
+                    seq_order, group_starts, shared_lens)
+    if shared_lens.dtype != torch.int32 or shared_lens.shape != (a.b,) or \
+            not shared_lens.is_contiguous():
+        raise ValueError("shared_lens must be contiguous int32 [num_seqs]")
+    if group_starts.dtype != torch.int32 or group_starts.dim() != 1 or \
+            group_starts.shape[0] < 1 or not group_starts.is_contiguous():
+        raise ValueError("group_starts must be contiguous int32 [num_groups + 1]")
+    if workspace is None:
+        need = decode_shared_workspace_bytes(a.b, a.hq, a.d, a.bs, a.max_blocks, int(max_shared),
+                                             int(split_keys), int(split_tokens))
+        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=a.dev)
+        a.ws_ptr, a.ws_bytes = workspace.data_ptr(), workspace.numel()
+    with _on(a.dev):
+        st = _lib.load().ps_paged_decode_shared(
+            a.out.data_ptr(), a.os, query.data_ptr(), a.qs, k_pool.data_ptr(), v_pool.data_ptr(),
+            a.nb, block_tables.data_ptr(), a.bt_stride, ctx_lens.data_ptr(), a.b,
+            group_starts.data_ptr(), group_starts.shape[0] - 1, shared_lens.data_ptr(),
+            int(max_group), int(max_shared), a.hq, a.hkv, a.d, a.bs, a.max_blocks, float(scale),
+            int(split_keys), int(split_tokens), a.ws_ptr, a.ws_bytes, _dtype_code(query),
+            a.order_ptr, _err_ptr(device_error), _stream(a.dev),
+        )
+    _lib.check(st, "paged_decode_shared")
     return a.out
 
 

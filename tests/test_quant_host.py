@@ -117,3 +117,42 @@ def test_quant_pools_are_checked():
                 (kp, kp, sc, sc.double()), (kp, kp, sc.transpose(0, 2), sc), (kp[0], kp, sc, sc)):
         with pytest.raises(ValueError):
             ops._check_quant_pools(*bad)
+
+
+def _shared(**kw):
+    a = dict(b=4, starts=16, groups=2, shared=16, max_group=2, max_shared=64, hq=8, hkv=2, d=128, bs=16, mb=8,
+             split_keys=0, split=0, ws=256, wsb=1 << 30, dtype=2)
+    a.update(kw)
+    return _lib.load().ps_paged_decode_shared(
+        16, 1024, 16, 1024, 16, 16, 8, 16, a["mb"], 16, a["b"], a["starts"], a["groups"], a["shared"],
+        a["max_group"], a["max_shared"], a["hq"], a["hkv"], a["d"], a["bs"], a["mb"], 0.1, a["split_keys"],
+        a["split"], a["ws"], a["wsb"], a["dtype"], None, None, None)
+
+
+def test_shared_refusals():
+    assert _shared(dtype=3) == _lib.PS_ERR_UNSUPPORTED
+    assert _shared(d=32) == _lib.PS_ERR_UNSUPPORTED
+    assert _shared(b=0) == _lib.PS_OK
+    assert _shared(max_shared=-1) == _lib.PS_ERR_INVALID
+    assert _shared(max_shared=129) == _lib.PS_ERR_INVALID and "max_shared" in _msg()
+    assert _shared(split_keys=64) == _lib.PS_ERR_INVALID
+    assert _shared(groups=5) == _lib.PS_ERR_INVALID
+    assert _shared(max_group=5) == _lib.PS_ERR_INVALID
+    assert _shared(starts=None) == _lib.PS_ERR_INVALID
+    assert _shared(shared=None) == _lib.PS_ERR_INVALID
+    assert _shared(ws=None) == _lib.PS_ERR_INVALID and "workspace" in _msg()
+    assert _shared(wsb=100) == _lib.PS_ERR_INVALID
+    assert _shared(ws=16) == _lib.PS_ERR_INVALID
+
+
+def test_shared_workspace_and_pieces():
+    size = ops.decode_shared_workspace_bytes
+    one = size(4, 8, 128, 16, 8, 64, 0, 0)
+    assert one == 4 * 8 * 128 * 4 + 4 * 8 * 8
+    assert size(4, 8, 128, 16, 80, 1280, 128, 0) == 10 * one
+    assert size(4, 8, 128, 16, 8, 0, 0, 0) == 0
+    assert size(4, 8, 128, 16, 8, 64, 0, 32) == one + ops.decode_workspace_bytes(4, 8, 128, 16, 8, 32)
+    # 256 rows x 4 heads = 4 pairs of tiles x 8 KV heads = 32 items over 8192 keys
+    keys = ops.shared_split_keys([256], 32, 8, 8192, 148)
+    assert keys % 128 == 0 and 32 * -(-8192 // keys) >= 0.8 * 148
+    assert ops.shared_split_keys([256], 32, 8, 128, 148) == 0
