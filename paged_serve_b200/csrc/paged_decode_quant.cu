@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(NW * 32)
     // 16 kk + 4 q4 .. + 3 of k step kk, as fp16 times 2^-e_head. The factor that
     // turns an S element of heads 2 q4, 2 q4 + 1 into log2 units goes to qs.
     uint32_t qb[kNT][kKSteps][2];
-    float qs[kNT][2];
+    float2 qs[kNT];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
       const bool real = nt * 8 + r < group;
@@ -236,37 +236,31 @@ __global__ void __launch_bounds__(NW * 32)
         qb[nt][kk][1] = pack2<__half>(x[kk][1].x * down, x[kk][1].y * down);
       }
       const float up = p.scale_log2 * pow2f(e);
-      qs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * q4);      // a lane of head 2 q4
-      qs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * q4 + 4);  // a lane of head 2 q4 + 1
+      qs[nt].x = __shfl_sync(0xffffffffu, up, 8 * q4);      // a lane of head 2 q4
+      qs[nt].y = __shfl_sync(0xffffffffu, up, 8 * q4 + 4);  // a lane of head 2 q4 + 1
     }
 
     float o[kNT][kKSteps][4];  // [dims 16 kk + 2 r (+1)][heads 2 q4, 2 q4 + 1]: {d0h0, d0h1, d1h0, d1h1}
     // Per head: running maxima of s (m) and s + log2 b (mv), the factor of P'
     // 2^(m - mv + 7), and this lane's part of the softmax sum.
-    float m[kNT][2], mv[kNT][2], f[kNT][2], l[kNT][2];
+    float2 m[kNT], mv[kNT], f[kNT], l[kNT];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
       for (int kk = 0; kk < kKSteps; ++kk) o[nt][kk][0] = o[nt][kk][1] = o[nt][kk][2] = o[nt][kk][3] = 0.f;
-      m[nt][0] = m[nt][1] = mv[nt][0] = mv[nt][1] = -INFINITY;
-      f[nt][0] = f[nt][1] = l[nt][0] = l[nt][1] = 0.f;
+      m[nt] = mv[nt] = make_float2(-INFINITY, -INFINITY);
+      f[nt] = l[nt] = make_float2(0.f, 0.f);
     }
     int stuck_at = -1;
 
     const int row8 = (lane & 7) + ((lane >> 3) & 1) * 8;  // ldmatrix: row of this lane's address
     const int chunk1 = lane >> 4;                         // and its 16-byte chunk (0 or 1)
 
-    for (int it = 0; warp + it * NW < nchunk; ++it) {
-      const int j = warp + it * NW;
-      const int st = warp * NS + (gbase + it) % NS;
-      if (!mbar_wait_bounded(&bars[st], ((gbase + it) / NS) & 1)) {
-        stuck_at = it;
-        break;
-      }
-      const uint32_t kbase = smem_u32(smem + st * 2 * SM::kTileBytes);
+    // One stage: kTail when fewer than 32 of its keys belong to the partition. A lane's
+    // two heads of a tile go through the softmax as packed pairs.
+    auto step = [&](auto tail, uint32_t kbase, const float* ks, int left) {
+      constexpr bool kTail = decltype(tail)::value;
       const uint32_t vbase = kbase + SM::kTileBytes;
-      const float* ks = reinterpret_cast<const float*>(smem + SM::kScaleOffset + st * 2 * kKeys * 4);
-      const int left = n_keys - j * kKeys;  // keys of the partition from this stage on
 
       // ---- S^T: two key tiles of 16
       float s[2][kNT][4];
@@ -274,8 +268,11 @@ __global__ void __launch_bounds__(NW * 32)
       for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) s[kt][nt][0] = s[kt][nt][1] = s[kt][nt][2] = s[kt][nt][3] = 0.f;
+      }
 #pragma unroll
-        for (int kk = 0; kk < kKSteps; kk += 2) {
+      for (int kk = 0; kk < kKSteps; kk += 2) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
           uint32_t w[4];
           ldsm_x4(kbase + SM::off(kt * 16 + row8, kk + chunk1), w[0], w[1], w[2], w[3]);
 #pragma unroll
@@ -292,13 +289,12 @@ __global__ void __launch_bounds__(NW * 32)
 
       // ---- scores in log2 units; this lane's keys are r, r + 8, r + 16, r + 24
       float vs[4];
-      float top[kNT][2], topv[kNT][2];
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) top[nt][0] = top[nt][1] = topv[nt][0] = topv[nt][1] = -INFINITY;
+      float2 x[4][kNT];
+      float2 top[kNT], topv[kNT];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = r + 8 * i;
-        const bool live = key < left;
+        const bool live = !kTail || key < left;
         const float a = ks[key];
         vs[i] = live ? ks[kKeys + key] : 0.f;
         // log2 b to within 0.09: the bits of a float, read as an integer, are linear
@@ -306,49 +302,48 @@ __global__ void __launch_bounds__(NW * 32)
         const float lb = fmaf(static_cast<float>(__float_as_int(vs[i])), 0x1p-23f, -127.f);
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& x = s[i >> 1][nt][(i & 1) * 2 + e];
-            x = live ? x * (a * qs[nt][e]) : -INFINITY;
-            top[nt][e] = fmaxf(top[nt][e], x);
-            topv[nt][e] = fmaxf(topv[nt][e], x + lb);
-          }
+          const float* sp = &s[i >> 1][nt][(i & 1) * 2];
+          x[i][nt] = __fmul2_rn(make_float2(sp[0], sp[1]), __fmul2_rn(make_float2(a, a), qs[nt]));
+          if (!live) x[i][nt] = make_float2(-INFINITY, -INFINITY);
+          const float2 y = __fadd2_rn(x[i][nt], make_float2(lb, lb));
+          top[nt].x = i ? fmaxf(top[nt].x, x[i][nt].x) : x[i][nt].x;
+          top[nt].y = i ? fmaxf(top[nt].y, x[i][nt].y) : x[i][nt].y;
+          topv[nt].x = i ? fmaxf(topv[nt].x, y.x) : y.x;
+          topv[nt].y = i ? fmaxf(topv[nt].y, y.y) : y.y;
         }
       }
       // ---- running maxima, moved only when passed by 2^8
       bool move = false;
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          move |= top[nt][e] > m[nt][e] + 8.f || topv[nt][e] > mv[nt][e] + 8.f;
-      }
+      for (int nt = 0; nt < kNT; ++nt)
+        move |= top[nt].x > m[nt].x + 8.f || top[nt].y > m[nt].y + 8.f ||
+                topv[nt].x > mv[nt].x + 8.f || topv[nt].y > mv[nt].y + 8.f;
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
-          float alpha[2];
+          auto raise = [&](float t, float u, float& m_, float& mv_, float& l_, float& f_) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float t = top[nt][e], u = topv[nt][e];
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-              u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, x));
+            for (int o_ = 4; o_ < 32; o_ <<= 1) {
+              t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o_));
+              u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, o_));
             }
-            const float m_new = fmaxf(m[nt][e], t);
-            const float mv_new = fmaxf(mv[nt][e], u);
-            l[nt][e] *= m_new == -INFINITY ? 1.f : ex2(m[nt][e] - m_new);
-            alpha[e] = mv_new == -INFINITY ? 1.f : ex2(mv[nt][e] - mv_new);
-            m[nt][e] = m_new;
-            mv[nt][e] = mv_new;
-            f[nt][e] = ex2(fminf(m_new - mv_new + 7.f, 120.f));
-          }
+            const float m_new = fmaxf(m_, t);
+            const float mv_new = fmaxf(mv_, u);
+            l_ *= m_new == -INFINITY ? 1.f : ex2(m_ - m_new);
+            const float alpha = mv_new == -INFINITY ? 1.f : ex2(mv_ - mv_new);
+            m_ = m_new;
+            mv_ = mv_new;
+            f_ = ex2(fminf(m_new - mv_new + 7.f, 120.f));
+            return alpha;
+          };
+          const float al0 = raise(top[nt].x, topv[nt].x, m[nt].x, mv[nt].x, l[nt].x, f[nt].x);
+          const float al1 = raise(top[nt].y, topv[nt].y, m[nt].y, mv[nt].y, l[nt].y, f[nt].y);
 #pragma unroll
           for (int kk = 0; kk < kKSteps; ++kk) {
-            o[nt][kk][0] *= alpha[0];
-            o[nt][kk][1] *= alpha[1];
-            o[nt][kk][2] *= alpha[0];
-            o[nt][kk][3] *= alpha[1];
+            o[nt][kk][0] *= al0;
+            o[nt][kk][1] *= al1;
+            o[nt][kk][2] *= al0;
+            o[nt][kk][3] *= al1;
           }
         }
       }
@@ -359,11 +354,11 @@ __global__ void __launch_bounds__(NW * 32)
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
-          const float p0 = ex2(s[i >> 1][nt][(i & 1) * 2] - m[nt][0]);
-          const float p1 = ex2(s[i >> 1][nt][(i & 1) * 2 + 1] - m[nt][1]);
-          l[nt][0] += p0;
-          l[nt][1] += p1;
-          pb[i >> 1][nt][i & 1] = transpose8x8(pack2<__half>(p0 * (vs[i] * f[nt][0]), p1 * (vs[i] * f[nt][1])));
+          const float2 z = __fadd2_rn(x[i][nt], make_float2(-m[nt].x, -m[nt].y));
+          const float2 pr = make_float2(ex2(z.x), ex2(z.y));
+          l[nt] = __fadd2_rn(l[nt], pr);
+          pb[i >> 1][nt][i & 1] = transpose8x8(
+              pack2<__half>(__fmul2_rn(pr, __fmul2_rn(make_float2(vs[i], vs[i]), f[nt]))));
         }
       }
 
@@ -374,7 +369,7 @@ __global__ void __launch_bounds__(NW * 32)
         // among it) must not meet a probability of 0. This lane's keys are
         // 2 q4, 2 q4 + 1 (low and high half of a register) and the same plus 8.
         uint32_t live0 = 0xffffffffu, live1 = 0xffffffffu;
-        if (left < kKeys) {
+        if constexpr (kTail) {
           const int k0 = left - kt * 16 - 2 * q4;
           live0 = k0 >= 2 ? 0xffffffffu : k0 == 1 ? 0x0000ffffu : 0u;
           live1 = k0 >= 10 ? 0xffffffffu : k0 == 9 ? 0x0000ffffu : 0u;
@@ -384,18 +379,34 @@ __global__ void __launch_bounds__(NW * 32)
           uint32_t w[4];
           ldsm_x4_t(vbase + SM::off(kt * 16 + row8, kk + chunk1), w[0], w[1], w[2], w[3]);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
+          for (int x2 = 0; x2 < 2; ++x2) {
             // bytes (key0 dim0, key0 dim1, key1 dim0, key1 dim1) -> pairs of keys per dim
             uint32_t a0, a1, a2, a3;
-            decode4<C>(__byte_perm(w[2 * x] & live0, 0, 0x3120), a0, a1);
-            decode4<C>(__byte_perm(w[2 * x + 1] & live1, 0, 0x3120), a2, a3);
+            if constexpr (kTail) {
+              w[2 * x2] &= live0;
+              w[2 * x2 + 1] &= live1;
+            }
+            decode4<C>(__byte_perm(w[2 * x2], 0, 0x3120), a0, a1);
+            decode4<C>(__byte_perm(w[2 * x2 + 1], 0, 0x3120), a2, a3);
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt)
-              Mma<__half>::run(o[nt][kk + x], a0, a1, a2, a3, pb[kt][nt][0], pb[kt][nt][1]);
+              Mma<__half>::run(o[nt][kk + x2], a0, a1, a2, a3, pb[kt][nt][0], pb[kt][nt][1]);
           }
         }
       }
+    };
 
+    for (int it = 0; warp + it * NW < nchunk; ++it) {
+      const int st = warp * NS + (gbase + it) % NS;
+      if (!mbar_wait_bounded(&bars[st], ((gbase + it) / NS) & 1)) {
+        stuck_at = it;
+        break;
+      }
+      const uint32_t kbase = smem_u32(smem + st * 2 * SM::kTileBytes);
+      const float* ks = reinterpret_cast<const float*>(smem + SM::kScaleOffset + st * 2 * kKeys * 4);
+      const int left = n_keys - (warp + it * NW) * kKeys;  // keys of the partition from here on
+      if (left >= kKeys) step(std::false_type{}, kbase, ks, left);
+      else step(std::true_type{}, kbase, ks, left);
       __syncwarp();
       if (warp + (it + NS) * NW < nchunk) {
         fence_proxy_async_smem();  // our reads of this stage precede the refill
@@ -425,14 +436,15 @@ __global__ void __launch_bounds__(NW * 32)
     for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float t = l[nt][e];  // each lane summed its own keys
+        float t = e ? l[nt].y : l[nt].x;  // each lane summed its own keys
         t += __shfl_xor_sync(0xffffffffu, t, 4);
         t += __shfl_xor_sync(0xffffffffu, t, 8);
         t += __shfl_xor_sync(0xffffffffu, t, 16);
         const int head = nt * 8 + 2 * q4 + e;
-        const float unit = f[nt][e] > 0.f ? 1.f / f[nt][e] : 0.f;  // O / f is in units of 2^m, like l
+        const float fe = e ? f[nt].y : f[nt].x;
+        const float unit = fe > 0.f ? 1.f / fe : 0.f;  // O / f is in units of 2^m, like l
         if (r == 0) {
-          ms[warp * R + head] = m[nt][e];
+          ms[warp * R + head] = e ? m[nt].y : m[nt].x;
           ls[warp * R + head] = t;
         }
 #pragma unroll
