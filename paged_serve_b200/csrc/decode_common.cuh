@@ -269,6 +269,37 @@ int reserve_smem(K kern, size_t smem, size_t (&configured)[64]) {
   return PS_OK;
 }
 
+// CTAs of a persistent launch: what one SM holds of `kern` with this many threads
+// and this much dynamic shared memory, and the SMs. `cache` (64 devices) belongs
+// to the kernel: kernels of one signature are one type here.
+struct Resident {
+  size_t smem = 0;
+  int per_sm = 0;
+  int sms = 0;
+};
+
+template <typename K>
+int resident_ctas(K kern, const char* fn, int threads, size_t smem, Resident (&cache)[64],
+                  Resident* out) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lock(g_launch_mu);
+  Resident fresh;
+  Resident& r = dev >= 0 && dev < 64 ? cache[dev] : fresh;
+  if (r.per_sm == 0 || r.smem != smem) {
+    int n = 0, count = 0;
+    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, smem);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess || n <= 0)
+      return fail(PS_ERR_CUDA, "%s: occupancy query failed: %s", fn, cudaGetErrorString(e));
+    r.smem = smem;
+    r.per_sm = n;
+    r.sms = count;
+  }
+  *out = r;
+  return PS_OK;
+}
+
 // Argument checks shared by every decode entry point; on success fills the
 // partition length (tokens), the partitions per sequence and the block-table
 // window a partition spans. Returns PS_OK, or the status of the first failure

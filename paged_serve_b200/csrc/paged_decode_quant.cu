@@ -526,18 +526,17 @@ int launch_quant(const QuantDecodeParams& qp, const CUtensorMap& km, const CUten
   static size_t configured[64] = {};
   int st = reserve_smem(kern, smem, configured);
   if (st != PS_OK) return st;
-  int dev = 0, sms = 148, per_sm = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kNW * 32, smem);
-  if (e != cudaSuccess || per_sm <= 0)
-    return fail(PS_ERR_CUDA, "%s: occupancy query failed: %s", fn, cudaGetErrorString(e));
+  static Resident cache[64];
+  Resident res;
+  st = resident_ctas(kern, fn, kNW * 32, smem, cache, &res);
+  if (st != PS_OK) return st;
+  cudaError_t e = cudaSuccess;
   if (!p.planned) {
     e = launch_pdl(decode_plan_kernel<false>, dim3(1), dim3(1024), 0, s, p);
     if (e != cudaSuccess)
       return fail(PS_ERR_CUDA, "%s(plan): launch failed: %s", fn, cudaGetErrorString(e));
   }
-  e = launch_pdl(kern, dim3(per_sm * sms), dim3(kNW * 32), smem, s, qp, km, vm);
+  e = launch_pdl(kern, dim3(res.per_sm * res.sms), dim3(kNW * 32), smem, s, qp, km, vm);
   if (e != cudaSuccess) return fail(PS_ERR_CUDA, "%s: launch failed: %s", fn, cudaGetErrorString(e));
   const int warps = p.num_launch * p.num_q_heads;
   e = launch_pdl(decode_combine_kernel<T, D>, dim3((warps + 3) / 4), dim3(128), 0, s, p);

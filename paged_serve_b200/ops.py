@@ -10,7 +10,6 @@ KV pool layout (per layer): ``[num_blocks, num_kv_heads, block_size, head_dim]``
 
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
@@ -51,29 +50,33 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
-    dev = None
+    first, index = None, -2
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError("paged_serve_b200 kernels need CUDA tensors (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} vs {t.device}")
-    assert dev is not None
-    return dev
+        i = t.get_device()  # -1 on the CPU; cheaper than comparing device objects
+        if i != index:
+            if i < 0:
+                raise ValueError("paged_serve_b200 kernels need CUDA tensors (no CPU fallback)")
+            if first is not None:
+                raise ValueError(f"tensors on different devices: {first.device} vs {t.device}")
+            first, index = t, i
+    assert first is not None
+    return first.device
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # The handle of torch.cuda.current_stream(device) without making a Stream object
+    # (3.8 us of host time a call).
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _on(device: torch.device):
-    """Makes ``device`` current for a launch (a no-op where it already is)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(device: torch.device, fn, *args) -> int:
+    """Calls ``fn`` with ``device`` current (the runtime launches on the current device)."""
+    if device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -81,17 +84,19 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _check_pool(pool: torch.Tensor, name: str) -> None:
-    if pool.dim() != 4 or not pool.is_contiguous():
+    if len(pool.shape) != 4 or not pool.is_contiguous():
         raise ValueError(f"{name} must be a contiguous [num_blocks, kv_heads, block_size, head_dim]")
 
 
 def _check_rows(x: torch.Tensor, name: str, heads: int, head_dim: int) -> int:
     """x is [rows, heads, head_dim] with unit dim stride and head stride head_dim."""
-    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != head_dim:
-        raise ValueError(f"{name} must be [rows, {heads}, {head_dim}], got {tuple(x.shape)}")
-    if x.stride(2) != 1 or x.stride(1) != head_dim:
+    shape = x.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
+        raise ValueError(f"{name} must be [rows, {heads}, {head_dim}], got {tuple(shape)}")
+    row, head, unit = x.stride()
+    if unit != 1 or head != head_dim:
         raise ValueError(f"{name} must have contiguous heads (strides (*, {head_dim}, 1))")
-    return x.stride(0) if x.shape[0] > 1 else heads * head_dim
+    return row if shape[0] > 1 else heads * head_dim
 
 
 def _err_ptr(device_error: torch.Tensor | None) -> int | None:
@@ -186,14 +191,17 @@ def _check_quant_pools(k_pool, v_pool, k_scale, v_scale) -> int:
     """Checks an 8-bit cache's pools and scales; returns their code type."""
     _check_pool(k_pool, "k_pool")
     _check_pool(v_pool, "v_pool")
-    if k_pool.dtype not in CODES:
-        raise ValueError(f"an 8-bit cache holds float8_e4m3fn or int8 codes, not {k_pool.dtype}")
-    if v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype:
+    dtype, shape = k_pool.dtype, k_pool.shape
+    code = CODES.get(dtype)
+    if code is None:
+        raise ValueError(f"an 8-bit cache holds float8_e4m3fn or int8 codes, not {dtype}")
+    if v_pool.shape != shape or v_pool.dtype != dtype:
         raise ValueError("k_pool/v_pool must share shape and dtype")
+    rows = shape[:3]
     for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        if t.dtype != torch.float32 or t.shape != k_pool.shape[:3] or not t.is_contiguous():
+        if t.dtype != torch.float32 or t.shape != rows or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous float32 [num_blocks, kv_heads, block_size]")
-    return CODES[k_pool.dtype]
+    return code
 
 
 def _append_quant(what, k_pool, v_pool, k_scale, v_scale, key, value, slot_mapping, positions,
@@ -213,22 +221,20 @@ def _append_quant(what, k_pool, v_pool, k_scale, v_scale, key, value, slot_mappi
         raise ValueError("slot_mapping must be contiguous")
     pools = (k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
              key.data_ptr(), value.data_ptr(), slot_mapping.data_ptr())
-    geometry = (t, ks, vs, hkv, d, bs, nb)
     tail = (_dtype_code(key), code, _err_ptr(device_error), _stream(dev))
     lib = _lib.load()
-    with _on(dev):
-        if positions is None:
-            st = lib.ps_cache_append_quant(*pools, *geometry, *tail)
-        else:
-            if positions.shape != (t,) or positions.dtype != torch.int64 or \
-                    not positions.is_contiguous():
-                raise ValueError("positions must be contiguous int64 [num_tokens]")
-            if (cos_sin_table.dim() != 2 or cos_sin_table.shape[1] != d
-                    or cos_sin_table.dtype != key.dtype or not cos_sin_table.is_contiguous()):
-                raise ValueError(f"cos_sin_table must be contiguous [positions, {d}] of the key dtype")
-            st = lib.ps_cache_append_rope_quant(
-                *pools, positions.data_ptr(), *geometry, cos_sin_table.data_ptr(),
-                cos_sin_table.shape[0], d, *tail)
+    if positions is None:
+        st = _launch(dev, lib.ps_cache_append_quant, *pools, t, ks, vs, hkv, d, bs, nb, *tail)
+    else:
+        if positions.shape != (t,) or positions.dtype != torch.int64 or \
+                not positions.is_contiguous():
+            raise ValueError("positions must be contiguous int64 [num_tokens]")
+        table_shape = cos_sin_table.shape
+        if (len(table_shape) != 2 or table_shape[1] != d or cos_sin_table.dtype != key.dtype
+                or not cos_sin_table.is_contiguous()):
+            raise ValueError(f"cos_sin_table must be contiguous [positions, {d}] of the key dtype")
+        st = _launch(dev, lib.ps_cache_append_rope_quant, *pools, positions.data_ptr(), t, ks, vs,
+                     hkv, d, bs, nb, cos_sin_table.data_ptr(), table_shape[0], d, *tail)
     _lib.check(st, what)
 
 
@@ -320,14 +326,13 @@ def cache_read_quant(
     w = block_tables.shape[1]
     if b == 0 or w == 0:
         return
-    with _on(dev):
-        st = _lib.load().ps_cache_read_quant(
-            k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nb,
-            k_out.data_ptr(), v_out.data_ptr(), k_out.shape[0], block_tables.data_ptr(),
-            block_tables.stride(0) if b > 1 else w, out_tables.data_ptr(),
-            out_tables.stride(0) if b > 1 else w, ctx_lens.data_ptr(), b, hkv, d, bs, w,
-            _dtype_code(k_out), code, _err_ptr(device_error), _stream(dev),
-        )
+    st = _launch(
+        dev, _lib.load().ps_cache_read_quant, k_pool.data_ptr(), v_pool.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), nb, k_out.data_ptr(), v_out.data_ptr(),
+        k_out.shape[0], block_tables.data_ptr(), block_tables.stride(0) if b > 1 else w,
+        out_tables.data_ptr(), out_tables.stride(0) if b > 1 else w, ctx_lens.data_ptr(), b, hkv, d,
+        bs, w, _dtype_code(k_out), code, _err_ptr(device_error), _stream(dev),
+    )
     _lib.check(st, "cache_read_quant")
 
 
@@ -544,11 +549,13 @@ class _DecodeArgs:
                  device_error, seq_order, *extra, quantised=False):
         self.dev = _require_cuda(query, k_pool, v_pool, block_tables, ctx_lens, out, workspace,
                                  device_error, seq_order, *extra)
-        _check_pool(k_pool, "k_pool")
-        _check_pool(v_pool, "v_pool")
-        self.nb, self.hkv, self.bs, self.d = k_pool.shape
-        d = self.d
-        if v_pool.shape != k_pool.shape or (query.dtype != k_pool.dtype and not quantised):
+        if not quantised:  # the caller checks an 8-bit cache's pools with their scales
+            _check_pool(k_pool, "k_pool")
+            _check_pool(v_pool, "v_pool")
+        shape, dtype = k_pool.shape, query.dtype
+        self.nb, self.hkv, self.bs, d = shape
+        self.d = d
+        if not quantised and (v_pool.shape != shape or dtype != k_pool.dtype):
             raise ValueError("k_pool/v_pool/query must share shape and dtype")
         if query.dim() != 3:
             raise ValueError("query must be [num_seqs, num_q_heads, head_dim]")
@@ -556,28 +563,33 @@ class _DecodeArgs:
         self.b, self.hq = b, hq
         self.qs = _check_rows(query, "query", hq, d)
         if out is None:
-            out = torch.empty((b, hq, d), dtype=query.dtype, device=self.dev)
-        if out.shape != (b, hq, d) or out.dtype != query.dtype:
-            raise ValueError("out must be [num_seqs, num_q_heads, head_dim] of the query dtype")
-        self.out = out
-        self.os = _check_rows(out, "out", hq, d)
-        if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or \
-                block_tables.shape[0] != b:
+            self.out = query.new_empty((b, hq, d))
+            self.os = hq * d
+        else:
+            if out.shape != (b, hq, d) or out.dtype != dtype:
+                raise ValueError("out must be [num_seqs, num_q_heads, head_dim] of the query dtype")
+            self.out = out
+            self.os = _check_rows(out, "out", hq, d)
+        table_shape = block_tables.shape
+        if block_tables.dtype != torch.int32 or len(table_shape) != 2 or table_shape[0] != b:
             raise ValueError("block_tables must be int32 [num_seqs, max_blocks]")
-        if block_tables.stride(1) != 1:
+        row, unit = block_tables.stride()
+        if unit != 1:
             raise ValueError("block_tables rows must be contiguous")
         if ctx_lens.dtype != torch.int32 or ctx_lens.shape != (b,) or not ctx_lens.is_contiguous():
             raise ValueError("ctx_lens must be contiguous int32 [num_seqs]")
-        if seq_order is not None and (seq_order.dtype != torch.int32 or seq_order.shape != (b,)
-                                      or not seq_order.is_contiguous()):
-            raise ValueError("seq_order must be contiguous int32 [num_seqs]")
-        self.max_blocks = block_tables.shape[1]
-        self.bt_stride = block_tables.stride(0) if b > 1 else self.max_blocks
+        self.order_ptr = None
+        if seq_order is not None:
+            if seq_order.dtype != torch.int32 or seq_order.shape != (b,) or \
+                    not seq_order.is_contiguous():
+                raise ValueError("seq_order must be contiguous int32 [num_seqs]")
+            self.order_ptr = seq_order.data_ptr()
+        self.max_blocks = table_shape[1]
+        self.bt_stride = row if b > 1 else self.max_blocks
         self.ws_ptr, self.ws_bytes = None, 0
         if workspace is not None:
             self.ws_ptr = workspace.data_ptr()
-            self.ws_bytes = workspace.numel() * workspace.element_size()
-        self.order_ptr = seq_order.data_ptr() if seq_order is not None else None
+            self.ws_bytes = workspace.nbytes
 
 
 def paged_decode(
@@ -673,9 +685,9 @@ def paged_decode_quant(
     these sequences, as in :func:`paged_decode_listed` (not with ``seq_order`` or
     ``planned``). Keys past a sequence's length are ignored whatever their rows hold.
     """
+    code = _check_quant_pools(k_pool, v_pool, k_scale, v_scale)
     a = _DecodeArgs(query, k_pool, v_pool, block_tables, ctx_lens, out, workspace, device_error,
                     seq_order, seq_list, k_scale, v_scale, quantised=True)
-    code = _check_quant_pools(k_pool, v_pool, k_scale, v_scale)
     listed, list_ptr = -1, a.order_ptr
     if seq_list is not None:
         if seq_order is not None or planned:
@@ -684,14 +696,13 @@ def paged_decode_quant(
             raise ValueError("seq_list must be contiguous int32 [n]")
         listed = seq_list.shape[0]
         list_ptr = seq_list.data_ptr() if listed else None
-    with _on(a.dev):
-        st = _lib.load().ps_paged_decode_quant(
-            a.out.data_ptr(), a.os, query.data_ptr(), a.qs, k_pool.data_ptr(), v_pool.data_ptr(),
-            k_scale.data_ptr(), v_scale.data_ptr(), a.nb, block_tables.data_ptr(), a.bt_stride,
-            ctx_lens.data_ptr(), a.b, list_ptr, listed, a.hq, a.hkv, a.d, a.bs, a.max_blocks,
-            float(scale), int(split_tokens), int(planned), a.ws_ptr, a.ws_bytes,
-            _dtype_code(query), code, _err_ptr(device_error), _stream(a.dev),
-        )
+    st = _launch(
+        a.dev, _lib.load().ps_paged_decode_quant, a.out.data_ptr(), a.os, query.data_ptr(), a.qs,
+        k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), a.nb,
+        block_tables.data_ptr(), a.bt_stride, ctx_lens.data_ptr(), a.b, list_ptr, listed, a.hq,
+        a.hkv, a.d, a.bs, a.max_blocks, float(scale), int(split_tokens), int(planned), a.ws_ptr,
+        a.ws_bytes, _dtype_code(query), code, _err_ptr(device_error), _stream(a.dev),
+    )
     _lib.check(st, "paged_decode_quant")
     return a.out
 
@@ -762,15 +773,14 @@ def paged_decode_shared(
                                              int(split_keys), int(split_tokens))
         workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=a.dev)
         a.ws_ptr, a.ws_bytes = workspace.data_ptr(), workspace.numel()
-    with _on(a.dev):
-        st = _lib.load().ps_paged_decode_shared(
-            a.out.data_ptr(), a.os, query.data_ptr(), a.qs, k_pool.data_ptr(), v_pool.data_ptr(),
-            a.nb, block_tables.data_ptr(), a.bt_stride, ctx_lens.data_ptr(), a.b,
-            group_starts.data_ptr(), group_starts.shape[0] - 1, shared_lens.data_ptr(),
-            int(max_group), int(max_shared), a.hq, a.hkv, a.d, a.bs, a.max_blocks, float(scale),
-            int(split_keys), int(split_tokens), a.ws_ptr, a.ws_bytes, _dtype_code(query),
-            a.order_ptr, _err_ptr(device_error), _stream(a.dev),
-        )
+    st = _launch(
+        a.dev, _lib.load().ps_paged_decode_shared, a.out.data_ptr(), a.os, query.data_ptr(), a.qs,
+        k_pool.data_ptr(), v_pool.data_ptr(), a.nb, block_tables.data_ptr(), a.bt_stride,
+        ctx_lens.data_ptr(), a.b, group_starts.data_ptr(), group_starts.shape[0] - 1,
+        shared_lens.data_ptr(), int(max_group), int(max_shared), a.hq, a.hkv, a.d, a.bs,
+        a.max_blocks, float(scale), int(split_keys), int(split_tokens), a.ws_ptr, a.ws_bytes,
+        _dtype_code(query), a.order_ptr, _err_ptr(device_error), _stream(a.dev),
+    )
     _lib.check(st, "paged_decode_shared")
     return a.out
 
