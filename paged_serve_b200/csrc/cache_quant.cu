@@ -38,33 +38,46 @@ __device__ __forceinline__ float row_max(float m) {
   return m;
 }
 
+// max |x| of eight values as two packed maxima (NaN when any is).
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = unpack2<T>(w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
+__device__ __forceinline__ float max_abs8(const uint4& v);
+template <>
+__device__ __forceinline__ float max_abs8<__nv_bfloat16>(const uint4& v) {
+  const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(&v);
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(w[0]), __habs2(w[1])),
+                                       __hmax2_nan(__habs2(w[2]), __habs2(w[3])));
+  return max_nan(__low2float(m), __high2float(m));
+}
+template <>
+__device__ __forceinline__ float max_abs8<__half>(const uint4& v) {
+  const __half2* w = reinterpret_cast<const __half2*>(&v);
+  const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(w[0]), __habs2(w[1])),
+                                __hmax2_nan(__habs2(w[2]), __habs2(w[3])));
+  return max_nan(__low2float(m), __high2float(m));
 }
 
-// Quantises one thread's sixteen values of a row and writes its codes (and, from
-// the row's first thread, the scale).
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& v, float2 (&x)[4]) {
+  x[0] = unpack2<T>(v.x);
+  x[1] = unpack2<T>(v.y);
+  x[2] = unpack2<T>(v.z);
+  x[3] = unpack2<T>(v.w);
+}
+
+// Quantises one thread's sixteen values of a row, m the largest of their |x|, and
+// writes its codes (and, from the row's first thread, the scale).
 template <typename C, int D>
-__device__ __forceinline__ void quantise_row(const float (&lo)[8], const float (&hi)[8],
+__device__ __forceinline__ void quantise_row(float m, const float2 (&lo)[4], const float2 (&hi)[4],
                                              uint8_t* codes, float* scale_out, int c, bool store) {
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max_nan(m, max_nan(fabsf(lo[i]), fabsf(hi[i])));
   const float scale = row_scale<C>(row_max<D / 16>(m));
-  const float inv = __fdiv_rn(1.f, scale);
   if (!store) return;
+  const float inv = __frcp_rn(scale);
+  const float2 inv2 = make_float2(inv, inv);
   uint2 a, b;
-  a.x = encode4<C>(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv);
-  a.y = encode4<C>(lo[4] * inv, lo[5] * inv, lo[6] * inv, lo[7] * inv);
-  b.x = encode4<C>(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv);
-  b.y = encode4<C>(hi[4] * inv, hi[5] * inv, hi[6] * inv, hi[7] * inv);
+  a.x = encode4<C>(__fmul2_rn(lo[0], inv2), __fmul2_rn(lo[1], inv2));
+  a.y = encode4<C>(__fmul2_rn(lo[2], inv2), __fmul2_rn(lo[3], inv2));
+  b.x = encode4<C>(__fmul2_rn(hi[0], inv2), __fmul2_rn(hi[1], inv2));
+  b.y = encode4<C>(__fmul2_rn(hi[2], inv2), __fmul2_rn(hi[3], inv2));
   *reinterpret_cast<uint2*>(codes + c * 8) = a;
   *reinterpret_cast<uint2*>(codes + D / 2 + c * 8) = b;
   if (c == 0) *scale_out = scale;
@@ -86,20 +99,20 @@ __global__ void __launch_bounds__(256)
   const int c = static_cast<int>(chunk % kThreadsPerRow);
   // Rows never straddle num_chunks: a row's threads are all active or all past the end.
   bool store = chunk < num_chunks;
-  float klo[8] = {}, khi[8] = {}, vlo[8] = {}, vhi[8] = {};
+  uint4 k0 = {}, k1 = {}, v0 = {}, v1 = {}, cv = {}, sv = {};
   int64_t dst = 0;
   if (store) {
     const uint32_t t = p.div_heads.div(row);
     const int h = static_cast<int>(row - t * p.num_kv_heads);
     const int64_t slot = p.slots[t];
-    const T* k = static_cast<const T*>(p.key) + t * p.key_stride + static_cast<int64_t>(h) * D;
-    const T* v = static_cast<const T*>(p.value) + t * p.value_stride + static_cast<int64_t>(h) * D;
-    const uint4 k0 = __ldcs(reinterpret_cast<const uint4*>(k + c * 8));
-    const uint4 k1 = __ldcs(reinterpret_cast<const uint4*>(k + D / 2 + c * 8));
-    const uint4 v0 = __ldcs(reinterpret_cast<const uint4*>(v + c * 8));
-    const uint4 v1 = __ldcs(reinterpret_cast<const uint4*>(v + D / 2 + c * 8));
     int64_t pos = 0;
     if constexpr (kRope) pos = p.positions[t];
+    const T* k = static_cast<const T*>(p.key) + t * p.key_stride + static_cast<int64_t>(h) * D + c * 8;
+    const T* v = static_cast<const T*>(p.value) + t * p.value_stride + static_cast<int64_t>(h) * D + c * 8;
+    k0 = __ldcs(reinterpret_cast<const uint4*>(k));
+    k1 = __ldcs(reinterpret_cast<const uint4*>(k + D / 2));
+    v0 = __ldcs(reinterpret_cast<const uint4*>(v));
+    v1 = __ldcs(reinterpret_cast<const uint4*>(v + D / 2));
     if (slot < 0) {
       store = false;  // padding token
     } else if (slot >= p.num_slots) {
@@ -112,26 +125,38 @@ __global__ void __launch_bounds__(256)
       const uint32_t blk = p.div_block.div(static_cast<uint32_t>(slot));
       const int off = static_cast<int>(static_cast<uint32_t>(slot) - blk * p.block_size);
       dst = (static_cast<int64_t>(blk) * p.num_kv_heads + h) * p.block_size + off;
-      unpack8<T>(k0, klo);
-      unpack8<T>(k1, khi);
-      unpack8<T>(v0, vlo);
-      unpack8<T>(v1, vhi);
       if constexpr (kRope) {
         const T* cs = static_cast<const T*>(p.table) + pos * D + c * 8;
-        float co[8], si[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(cs), co);
-        unpack8<T>(*reinterpret_cast<const uint4*>(cs + D / 2), si);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float a = klo[i], b = khi[i];
-          klo[i] = __fsub_rn(__fmul_rn(a, co[i]), __fmul_rn(b, si[i]));
-          khi[i] = __fadd_rn(__fmul_rn(b, co[i]), __fmul_rn(a, si[i]));
-        }
+        cv = *reinterpret_cast<const uint4*>(cs);
+        sv = *reinterpret_cast<const uint4*>(cs + D / 2);
       }
     }
   }
-  quantise_row<C, D>(klo, khi, static_cast<uint8_t*>(p.k_pool) + dst * D, p.k_scale + dst, c, store);
-  quantise_row<C, D>(vlo, vhi, static_cast<uint8_t*>(p.v_pool) + dst * D, p.v_scale + dst, c, store);
+  float2 lo[4], hi[4];
+  unpack8<T>(v0, lo);
+  unpack8<T>(v1, hi);
+  quantise_row<C, D>(max_nan(max_abs8<T>(v0), max_abs8<T>(v1)), lo, hi,
+                     static_cast<uint8_t*>(p.v_pool) + dst * D, p.v_scale + dst, c, store);
+  unpack8<T>(k0, lo);
+  unpack8<T>(k1, hi);
+  float m = 0.f;
+  if constexpr (kRope) {
+    float2 co[4], si[4];
+    unpack8<T>(cv, co);
+    unpack8<T>(sv, si);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = lo[i], b = hi[i];
+      const float2 bs = __fmul2_rn(b, si[i]);  // exact, so the sums below round once
+      lo[i] = __ffma2_rn(a, co[i], make_float2(-bs.x, -bs.y));
+      hi[i] = __ffma2_rn(b, co[i], __fmul2_rn(a, si[i]));
+      m = max3_abs_nan(m, lo[i].x, lo[i].y);
+      m = max3_abs_nan(m, hi[i].x, hi[i].y);
+    }
+  } else {
+    m = max_nan(max_abs8<T>(k0), max_abs8<T>(k1));
+  }
+  quantise_row<C, D>(m, lo, hi, static_cast<uint8_t*>(p.k_pool) + dst * D, p.k_scale + dst, c, store);
 }
 
 template <typename T, int D, typename C, bool kRope>
@@ -235,15 +260,16 @@ struct ReadQuantParams {
   int64_t num_out_blocks;
   int max_blocks;
   int block_size;
-  int vecs;  // 16-code vectors of one block: num_kv_heads * block_size * head_dim / 16
+  int vecs;  // 8-code vectors of one block: num_kv_heads * block_size * head_dim / 8
   FastDiv div_block;
   int32_t* err;
 };
 
 // One CTA per (block of a sequence): a block's codes are contiguous, and so are
-// its values in the output block. A thread turns 16 codes of one row into 32
-// bytes; rows past the sequence's last token are written as zeros, so what a
-// freed block held before (NaN among it) never reaches a reader of whole tiles.
+// its values in the output block. A thread turns 8 codes of one row into 16 bytes
+// (16 codes into two 16-byte stores leave half of each sector to the second store), four
+// such loads in flight; rows past the sequence's last token are written as zeros, so what
+// a freed block held before (NaN among it) never reaches a reader of whole tiles.
 template <typename T, int D, typename C>
 __global__ void __launch_bounds__(256) cache_read_quant_kernel(const ReadQuantParams p) {
   pdl_trigger();
@@ -263,32 +289,45 @@ __global__ void __launch_bounds__(256) cache_read_quant_kernel(const ReadQuantPa
     if (threadIdx.x == 0) set_device_error(p.err, PS_DEVERR_BLOCK_ID);
     return;
   }
-  const int64_t rows = static_cast<int64_t>(p.vecs) * 16 / D;
-  for (int i = threadIdx.x; i < 2 * p.vecs; i += blockDim.x) {
-    const bool is_v = i >= p.vecs;
-    const int v = is_v ? i - p.vecs : i;
-    const uint32_t row = static_cast<uint32_t>(v) / (D / 16);  // head * block_size + offset
-    const int off = static_cast<int>(row - p.div_block.div(row) * p.block_size);
-    uint32_t out[8] = {};
-    if (off < left) {
-      const uint4 codes = __ldcs(reinterpret_cast<const uint4*>(
-          (is_v ? p.v_pool : p.k_pool) + (static_cast<int64_t>(src) * p.vecs + v) * 16));
-      const float scale = (is_v ? p.v_scale : p.k_scale)[src * rows + row];
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(&codes);
+  constexpr int kUnroll = 4;
+  const int64_t rows = static_cast<int64_t>(p.vecs) * 8 / D;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        uint32_t lo, hi;
-        decode4<C>(w[x], lo, hi);
-        const float2 f0 = unpack2<__half>(lo);
-        const float2 f1 = unpack2<__half>(hi);
-        out[2 * x] = pack2<T>(f0.x * scale, f0.y * scale);
-        out[2 * x + 1] = pack2<T>(f1.x * scale, f1.y * scale);
+  for (int is_v = 0; is_v < 2; ++is_v) {
+    const uint2* codes = reinterpret_cast<const uint2*>(is_v ? p.v_pool : p.k_pool) +
+                         static_cast<int64_t>(src) * p.vecs;
+    const float* scales = (is_v ? p.v_scale : p.k_scale) + src * rows;
+    uint4* out = reinterpret_cast<uint4*>(is_v ? p.v_out : p.k_out) +
+                 static_cast<int64_t>(dst) * p.vecs;
+    for (int i0 = threadIdx.x; i0 < p.vecs; i0 += kUnroll * 256) {
+      uint2 c[kUnroll];
+      float s[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int i = i0 + u * 256;
+        c[u] = make_uint2(0u, 0u);
+        s[u] = 0.f;
+        if (i < p.vecs) {
+          const uint32_t row = static_cast<uint32_t>(i) / (D / 8);  // head * block_size + offset
+          const int off = static_cast<int>(row - p.div_block.div(row) * p.block_size);
+          if (off < left) {
+            c[u] = __ldcs(codes + i);
+            s[u] = scales[row];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int i = i0 + u * 256;
+        uint32_t h[4];
+        decode4<C>(c[u].x, h[0], h[1]);
+        decode4<C>(c[u].y, h[2], h[3]);
+        uint32_t o[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          o[x] = pack2<T>(__fmul2_rn(unpack2<__half>(h[x]), make_float2(s[u], s[u])));
+        if (i < p.vecs) out[i] = make_uint4(o[0], o[1], o[2], o[3]);
       }
     }
-    uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(is_v ? p.v_out : p.k_out) +
-                                        (static_cast<int64_t>(dst) * p.vecs + v) * 16);
-    o[0] = make_uint4(out[0], out[1], out[2], out[3]);
-    o[1] = make_uint4(out[4], out[5], out[6], out[7]);
   }
 }
 
@@ -380,7 +419,7 @@ extern "C" int ps_cache_read_quant(const void* k_pool, const void* v_pool, const
   p.num_out_blocks = num_out_blocks;
   p.max_blocks = max_blocks_per_seq;
   p.block_size = block_size;
-  p.vecs = num_kv_heads * block_size * (head_dim / 16);
+  p.vecs = num_kv_heads * block_size * (head_dim / 8);
   p.div_block = FastDiv(static_cast<uint32_t>(block_size));
   p.err = device_error;
   const dim3 grid(static_cast<unsigned>(max_blocks_per_seq), static_cast<unsigned>(num_seqs));

@@ -60,15 +60,36 @@ struct DecodeParams {
   const int64_t* new_slots;
   int64_t num_slots;
   // Optional shared prefix (ps_paged_decode_shared): the first shared_lens[b] keys of
-  // sequence b are attended by the prefix pass, which leaves pieces of pre_keys keys
-  // as unnormalised outputs pre_o and (running max, sum) pre_ml, rows
-  // (piece * num_seqs + b) * num_q_heads + head. Partitions cut the keys behind them.
+  // sequence b are attended by the prefix pass, which leaves pre_parts partials per piece
+  // of pre_keys keys in pre_o and pre_ml (laid out as in shared_prefix.h). Partitions
+  // cut the keys behind them.
   const int32_t* shared_lens;
   const float* pre_o;
   const float2* pre_ml;
   int pre_keys;
+  int pre_parts;
   int pre_max;  // largest prefix the pieces hold
 };
+
+// Partials of a shared prefix: their number for a prefix of `pre` keys, and where a
+// row's start (float4 columns for pre_o, 32 apart; rows for pre_ml).
+struct SharedRows {
+  int64_t row, blocks;
+  __device__ __forceinline__ SharedRows(const DecodeParams& p, int b, int h, int g)
+      : row((static_cast<int64_t>(h) * p.num_seqs + b) * p.group + g),
+        blocks((static_cast<int64_t>(p.num_seqs) * p.num_q_heads + 31) / 32) {}
+  __device__ __forceinline__ float2 ml(const DecodeParams& p, int part) const {
+    return p.pre_ml[part * blocks * 32 + row];
+  }
+  template <int D>
+  __device__ __forceinline__ float4 o(const DecodeParams& p, int part, int col4) const {
+    return reinterpret_cast<const float4*>(
+        p.pre_o)[((part * blocks + row / 32) * (D / 4) + col4) * 32 + row % 32];
+  }
+};
+__device__ __forceinline__ int shared_parts(const DecodeParams& p, int pre) {
+  return pre > 0 ? (pre + p.pre_keys - 1) / p.pre_keys * p.pre_parts : 0;
+}
 
 // Shared-prefix tokens of sequence b with ctx keys; 0 (and an error bit) when
 // the prefix is not whole blocks of the sequence or longer than the pieces hold.
@@ -176,10 +197,9 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const DecodeParams 
   float mmax = -INFINITY;
   for (int s = lane; s < nsplit; s += 32)
     mmax = fmaxf(mmax, p.ws_lse[base + static_cast<int64_t>(s) * p.num_q_heads]);
-  const int npre = kShared && pre > 0 ? (pre + p.pre_keys - 1) / p.pre_keys : 0;
-  const int64_t pre_row = static_cast<int64_t>(b) * p.num_q_heads + qh;
-  const int64_t pre_step = static_cast<int64_t>(p.num_seqs) * p.num_q_heads;
-  for (int s = lane; s < npre; s += 32) mmax = fmaxf(mmax, p.pre_ml[pre_row + s * pre_step].x);
+  const int npre = kShared ? shared_parts(p, pre) : 0;
+  const SharedRows shared(p, b, qh / p.group, qh % p.group);
+  for (int s = lane; s < npre; s += 32) mmax = fmaxf(mmax, shared.ml(p, s).x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mmax = fmaxf(mmax, __shfl_xor_sync(0xffffffffu, mmax, o));
   constexpr int kPer = D / 32;  // dims per lane
@@ -229,12 +249,14 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const DecodeParams 
     }
     for (; k < n; ++k) add(__shfl_sync(0xffffffffu, wl, k), load(s0 + k));
   }
+#pragma unroll 8
   for (int s = 0; s < npre; ++s) {
-    const int64_t row = pre_row + s * pre_step;
-    const float2 ml = p.pre_ml[row];
+    const float2 ml = shared.ml(p, s);
     const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mmax);
     wsum += w * (ml.y - 1.f);  // add() counts the weight once
-    add(w, *reinterpret_cast<const Vec*>(p.pre_o + row * D + lane * kPer));
+    const float4 v = shared.o<D>(p, s, lane * kPer / 4);
+    if constexpr (kPer == 4) add(w, v);
+    else add(w, lane & 1 ? make_float2(v.z, v.w) : make_float2(v.x, v.y));
   }
   const float inv = (wsum > 0.f) ? 1.f / wsum : 0.f;
   T* orow = static_cast<T*>(p.out) + b * p.out_stride + static_cast<int64_t>(qh) * D + lane * kPer;

@@ -424,17 +424,17 @@ __global__ void __launch_bounds__(NW * 32)
   // The prefix pass has left its pieces (and whatever runs after this kernel waits
   // for that pass too, since every CTA does).
   if constexpr (kShared) pdl_wait();
-  const int npre = kShared && single && pre > 0 ? (pre + p.pre_keys - 1) / p.pre_keys : 0;
+  const int npre = kShared && single ? shared_parts(p, pre) : 0;
   for (int idx = threadIdx.x; idx < group * (D / 4); idx += blockDim.x) {
-    const int g = idx / (D / 4);
-    const int d = (idx % (D / 4)) * 4;
+    // kShared: neighbouring lanes take the heads, whose rows of a partial are neighbours.
+    const int g = kShared ? idx % group : idx / (D / 4);
+    const int d = (kShared ? idx / group : idx % (D / 4)) * 4;
     float mmax = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) mmax = fmaxf(mmax, ms[w * R + g]);
-    const int64_t pre_row = static_cast<int64_t>(b) * p.num_q_heads + h * group + g;
-    const int64_t pre_step = static_cast<int64_t>(p.num_seqs) * p.num_q_heads;
+    const SharedRows shared(p, b, h, g);
     if constexpr (kShared) {
-      for (int s = 0; s < npre; ++s) mmax = fmaxf(mmax, p.pre_ml[pre_row + s * pre_step].x);
+      for (int s = 0; s < npre; ++s) mmax = fmaxf(mmax, shared.ml(p, s).x);
     }
     float lsum = 0.f;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -450,12 +450,11 @@ __global__ void __launch_bounds__(NW * 32)
       acc[3] += ov.w * sc;
     }
     if constexpr (kShared) {
-#pragma unroll 4
+#pragma unroll 8
       for (int s = 0; s < npre; ++s) {
-        const int64_t row = pre_row + s * pre_step;
-        const float2 ml = p.pre_ml[row];
+        const float2 ml = shared.ml(p, s);
+        const float4 ov = shared.o<D>(p, s, d / 4);
         const float sc = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mmax);
-        const float4 ov = *reinterpret_cast<const float4*>(p.pre_o + row * D + d);
         lsum += ml.y * sc;
         acc[0] += ov.x * sc;
         acc[1] += ov.y * sc;
@@ -802,6 +801,7 @@ int decode_entry(const char* fn, void* out, int64_t out_seq_stride, const void* 
     p.pre_o = shared->part_o;
     p.pre_ml = shared->part_ml;
     p.pre_keys = shared->piece_keys;
+    p.pre_parts = shared->paired ? 2 : 1;
     p.pre_max = shared->pieces * shared->piece_keys;
     return dispatch_decode<true>(p, km, vm, s, dtype, head_dim, block_size, shared);
   }
@@ -956,7 +956,10 @@ SharedLayout shared_layout(int num_seqs, int num_q_heads, int head_dim, int max_
   if (max_shared <= 0) return l;
   l.piece_keys = split_keys > 0 ? split_keys : (max_shared + 127) / 128 * 128;
   l.pieces = (max_shared + l.piece_keys - 1) / l.piece_keys;
-  const int64_t rows = static_cast<int64_t>(l.pieces) * num_seqs * num_q_heads;
+  // Room for two partials a piece: whether a piece leaves one or two depends on the
+  // groups' sizes, which the workspace should not.
+  const int64_t rows = 2 * static_cast<int64_t>(l.pieces) *
+                       ((static_cast<int64_t>(num_seqs) * num_q_heads + 31) / 32 * 32);
   l.o_bytes = (rows * head_dim * 4 + 255) / 256 * 256;
   l.ml_bytes = (rows * 8 + 255) / 256 * 256;
   return l;
@@ -1042,6 +1045,7 @@ extern "C" int ps_paged_decode_shared(
   a.max_blocks = max_blocks_per_seq;
   a.pieces = l.pieces;
   a.piece_keys = l.piece_keys;
+  a.paired = static_cast<int64_t>(max_group) * (num_q_heads / num_kv_heads) <= 128;
   a.scale = scale;
   a.part_o = reinterpret_cast<float*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + l.o_bytes);

@@ -349,7 +349,12 @@ __global__ void __launch_bounds__(NW * 32)
       }
 
       // ---- P^T as the B operand: [kt][nt][keys 0-7 | 8-15]
+      // P' is rounded to fp16: 2^-11 of a probability, an eighth of a bf16 output's own
+      // rounding but all of an fp16 output's. There a second fp16 term holds what the first
+      // one lost (one more MMA per tile; the tensor pipe is a fifth busy).
+      constexpr bool kTwoTerms = std::is_same<T, __half>::value;
       uint32_t pb[2][kNT][2];
+      [[maybe_unused]] uint32_t pl[2][kNT][2];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -357,8 +362,14 @@ __global__ void __launch_bounds__(NW * 32)
           const float2 z = __fadd2_rn(x[i][nt], make_float2(-m[nt].x, -m[nt].y));
           const float2 pr = make_float2(ex2(z.x), ex2(z.y));
           l[nt] = __fadd2_rn(l[nt], pr);
-          pb[i >> 1][nt][i & 1] = transpose8x8(
-              pack2<__half>(__fmul2_rn(pr, __fmul2_rn(make_float2(vs[i], vs[i]), f[nt]))));
+          const float2 pv = __fmul2_rn(pr, __fmul2_rn(make_float2(vs[i], vs[i]), f[nt]));
+          const uint32_t hi = pack2<__half>(pv);
+          pb[i >> 1][nt][i & 1] = transpose8x8(hi);
+          if constexpr (kTwoTerms) {
+            const float2 back = unpack2<__half>(hi);
+            pl[i >> 1][nt][i & 1] =
+                transpose8x8(pack2<__half>(__fadd2_rn(pv, make_float2(-back.x, -back.y))));
+          }
         }
       }
 
@@ -390,7 +401,11 @@ __global__ void __launch_bounds__(NW * 32)
             decode4<C>(__byte_perm(w[2 * x2 + 1], 0, 0x3120), a2, a3);
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt)
+            {
               Mma<__half>::run(o[nt][kk + x2], a0, a1, a2, a3, pb[kt][nt][0], pb[kt][nt][1]);
+              if constexpr (kTwoTerms)
+                Mma<__half>::run(o[nt][kk + x2], a0, a1, a2, a3, pl[kt][nt][0], pl[kt][nt][1]);
+            }
           }
         }
       }

@@ -95,6 +95,7 @@ struct Cfg {
 constexpr int kThreads = 384;
 constexpr int kWarpTma = 8;
 constexpr int kWarpMma = 9;
+constexpr int kWarpTmaV = 10;  // paired shared-prefix tiles only
 constexpr uint32_t kRegsSoftmax = 192;
 constexpr uint32_t kRegsOther = 64;
 constexpr int kRegPoolNeeded = 256 * kRegsSoftmax + 128 * kRegsOther;
@@ -133,7 +134,10 @@ struct PrefillParams {
   float2* part_ml;   // [num_units][2 tiles][128 rows] (running max, log2 units; row sum)
   // Shared-prefix pass of a decode step (kShared): a "sequence" is a group of
   // neighbouring batch rows, q_starts their group starts [num_seqs + 1], ctx_lens the
-  // shared prefix of each batch row; partials are [splits][num_rows][Hq] rows.
+  // shared prefix of each batch row. With `paired` (groups that fill one query tile at
+  // most) tiles A and B hold the same rows and take even and odd key tiles, so the
+  // softmax of one still runs beside the other's MMAs, and a piece leaves two partials.
+  bool paired;
   float scale_log2;
   int32_t* err;
 };
@@ -150,6 +154,7 @@ struct Item {
   int b, h, t0, q_len, ctx, q_start, ntiles, nblk_seq, last_key;
   int unit, j0;  // the unit (kShared: the piece), and its first key tile (0 unless split)
   bool partial;  // the item spans several pieces: write partials, not the output
+  int nload, j_last;  // kShared: key tiles to load, and the last one that exists
 };
 
 // False when the unit has no rows or no keys (or invalid lengths, which set an
@@ -182,12 +187,11 @@ __device__ __forceinline__ bool decode_item(const PrefillParams& p, int u, Item&
     w.q_len = p.q_starts[w.b + 1] - w.q_start;
     if (w.t0 >= w.q_len) return false;
     if (w.q_start < 0 || w.q_len > p.num_rows - w.q_start ||
-        w.q_len > nq * 2 * p.tokens_per_tile) {
+        w.q_len > nq * (p.paired ? 1 : 2) * p.tokens_per_tile) {
       if (report) set_device_error(p.err, PS_DEVERR_LENGTH);
       return false;
     }
     w.ctx = p.ctx_lens[w.q_start];
-    w.last_key = w.ctx;
     const int64_t room = static_cast<int64_t>(p.splits) * p.split_tiles * kN;  // pieces' keys
     if (w.ctx <= 0 || w.ctx > p.max_blocks * p.block_size || w.ctx > room ||
         w.ctx % p.block_size != 0) {
@@ -199,6 +203,10 @@ __device__ __forceinline__ bool decode_item(const PrefillParams& p, int u, Item&
     w.j0 = piece * p.split_tiles;
     if (w.j0 >= item_tiles) return false;
     w.ntiles = min(p.split_tiles, item_tiles - w.j0);
+    w.j_last = w.j0 + w.ntiles - 1;
+    w.last_key = min(w.ctx, (w.j_last + 1) * kN);  // keys of this piece end here
+    if (p.paired) w.ntiles = (w.ntiles + 1) / 2;
+    w.nload = p.paired ? 2 * w.ntiles : w.ntiles;
     w.partial = true;
     w.nblk_seq = w.ctx / p.block_size;
     return true;
@@ -298,7 +306,8 @@ __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* b
                                              int warp_in_tile, const Item& w, int g0, int n) {
   using C = Cfg<D>;
   const int ntiles = w.ntiles;
-  const int t0_tile = w.t0 + tile * p.tokens_per_tile;
+  const bool paired = kShared && p.paired;
+  const int t0_tile = w.t0 + (paired ? 0 : tile * p.tokens_per_tile);
   const int ctx = w.ctx, q_len = w.q_len, q_start = w.q_start, h = w.h, last_key = w.last_key;
   const int G = p.group;
   const int tpt = p.tokens_per_tile;
@@ -324,7 +333,7 @@ __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* b
     for (int c = 0; c < 4; ++c) tmem_ld32(lane_tmem + s_col + c * 32, sraw[c]);
     tmem_wait_ld();
     float* s = reinterpret_cast<float*>(&sraw[0][0]);
-    const int key0 = (w.j0 + j) * kN;
+    const int key0 = (w.j0 + (paired ? 2 * j + tile : j)) * kN;
     if (key0 + kN - 1 > tile_min_limit) {  // diagonal tile: causal mask (warp-uniform test)
 #pragma unroll
       for (int c = 0; c < kN; ++c)
@@ -416,22 +425,39 @@ __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* b
     for (int c = 0; c < D / 32; ++c) tmem_ld32(lane_tmem + o_col + c * 32, oall[c]);
     tmem_wait_ld();
     if (row_real) {
-      int64_t prow = (static_cast<int64_t>(w.unit) * 2 + tile) * kM + r;
       if constexpr (kShared) {
+        // Row (h, batch row, head) of 32-row blocks in which a column of four floats is
+        // contiguous over the rows: the rows of a tile are neighbours, so a warp's
+        // stores fill whole sectors (row by row they wrote half of each, and took
+        // longer than the key tile before them).
         const int row = q_start + t0_tile + tok;
-        prow = (static_cast<int64_t>(w.unit) * p.num_rows + row) * p.num_q_heads + h * G + r % G;
+        const int64_t prow = (static_cast<int64_t>(h) * p.num_rows + row) * G + r % G;
+        const int64_t blocks = (p.num_rows * p.num_q_heads + 31) / 32;
+        const int64_t piece = static_cast<int64_t>(w.unit) * (paired ? 2 : 1) + (paired ? tile : 0);
+        float4* po = reinterpret_cast<float4*>(p.part_o) +
+                     (piece * blocks + prow / 32) * (D / 4) * 32 + prow % 32;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+          for (int v = 0; v < 8; ++v)
+            po[(c * 8 + v) * 32] = make_float4(__uint_as_float(oall[c][4 * v]), __uint_as_float(oall[c][4 * v + 1]),
+                                               __uint_as_float(oall[c][4 * v + 2]), __uint_as_float(oall[c][4 * v + 3]));
+        }
+        p.part_ml[piece * blocks * 32 + prow] = make_float2(m_used, l_sum);
         // A row that names another length would merge pieces it does not have.
         if (p.ctx_lens[row] != ctx) set_device_error(p.err, PS_DEVERR_LENGTH);
-      }
-      float4* po = reinterpret_cast<float4*>(p.part_o + prow * D);
+      } else {
+        const int64_t prow = (static_cast<int64_t>(w.unit) * 2 + tile) * kM + r;
+        float4* po = reinterpret_cast<float4*>(p.part_o + prow * D);
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
+        for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
-        for (int v = 0; v < 8; ++v)
-          po[c * 8 + v] = make_float4(__uint_as_float(oall[c][4 * v]), __uint_as_float(oall[c][4 * v + 1]),
-                                      __uint_as_float(oall[c][4 * v + 2]), __uint_as_float(oall[c][4 * v + 3]));
+          for (int v = 0; v < 8; ++v)
+            po[c * 8 + v] = make_float4(__uint_as_float(oall[c][4 * v]), __uint_as_float(oall[c][4 * v + 1]),
+                                        __uint_as_float(oall[c][4 * v + 2]), __uint_as_float(oall[c][4 * v + 3]));
+        }
+        p.part_ml[prow] = make_float2(m_used, l_sum);
       }
-      p.part_ml[prow] = make_float2(m_used, l_sum);
     }
     tc_fence_before();
     return true;
@@ -511,7 +537,96 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Branch per warpgroup first, so each register budget covers exactly its code.
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-  if (warp == kWarpTma) {
+  if (kShared && p.paired && (warp == kWarpTma || warp == kWarpTmaV)) {
+    // ------------------------------------------------------------ TMA producers (paired)
+    // One warp loads Q and K, another V: a warp issues a copy in about 100 cycles, and a
+    // pair of key tiles is 64 copies with blocks of 16 (one warp for both: 3.4 us a pair
+    // against 2.1, one group of eight rows over 32768 keys in one piece). Each keeps the
+    // next 32 block ids in flight. Unpaired, the MMAs take longer than one warp's copies,
+    // and K before V in one warp's order is 7% faster.
+    if constexpr (kShared) {
+      const bool is_v = warp == kWarpTmaV;
+      const CUtensorMap* map = is_v ? &vmap : &kmap;
+      uint8_t* base = smem + (is_v ? C::kOffV : C::kOffK);
+      const int stages = is_v ? C::kVStages : C::kKStages;
+      const int bar_full = is_v ? C::kBarVFull : C::kBarKFull;
+      const int bar_empty = is_v ? C::kBarVEmpty : C::kBarKEmpty;
+      if (lane == 0) {
+        tma_prefetch_desc(&qmap);
+        tma_prefetch_desc(map);
+      }
+      int c = 0, n = 0;  // tiles and items issued so far
+      bool ok = true;
+      for (int it = blockIdx.x; ok && it < p.num_units; it += gridDim.x) {
+        Item w;
+        if (!decode_item<kSplit, kShared>(p, it, w, lane == 0 && !is_v)) continue;
+        const int32_t* bt = p.block_tables + static_cast<int64_t>(w.q_start) * p.bt_stride;
+        int window = w.j0 * kTileBlocks;  // first block of the 32 in the lanes
+        // Blocks past the prefix repeat its last one (their keys are masked).
+        auto load_id = [&](int from) { return bt[min(from + lane, w.nblk_seq - 1)]; };
+        int32_t id = load_id(window);
+        int32_t id_next = load_id(window + 32);
+        auto row_of = [&](int32_t x) {
+          if (x < 0 || x >= p.num_blocks) {
+            set_device_error(p.err, PS_DEVERR_BLOCK_ID);
+            x = 0;
+          }
+          return (x * p.num_kv_heads + w.h) * BS;
+        };
+        int32_t my_row = row_of(id);
+        for (int j = 0; ok && j < w.nload; ++j) {
+          // An odd last tile's partner re-reads it (all its keys are masked).
+          const int kb0 = min(w.j0 + j, w.j_last) * kTileBlocks;
+          if (kb0 >= window + 32) {  // a tile's blocks never straddle two windows
+            window += 32;
+            my_row = row_of(id_next);
+            id_next = load_id(window + 32);
+          }
+          const int st = c % stages;
+          if (lane == 0 && c >= stages)
+            ok = wait_or_abort(&bars[bar_empty + st], ((c / stages) - 1) & 1, abort, p.err);
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+          if (!ok) break;
+          uint8_t* dst = base + st * C::kKVBytes;
+          if (lane == 0) mbar_arrive_expect_tx(&bars[bar_full + st], C::kKVBytes);
+#pragma unroll
+          for (int bb = 0; bb < kTileBlocks; ++bb) {
+            const int32_t row = __shfl_sync(0xffffffffu, my_row, kb0 - window + bb);
+            if (lane == 0) {
+#pragma unroll
+              for (int hh = 0; hh < C::kHalves; ++hh)
+                tma_load_2d(dst + hh * kKVHalf + bb * (BS * 128), map, &bars[bar_full + st], 64 * hh, row);
+            }
+          }
+          ++c;
+          if (j == 0 && !is_v) {
+            if (lane == 0) {
+              if (n > 0) ok = wait_or_abort(&bars[C::kBarQFree], (n - 1) & 1, abort, p.err);
+              if (ok) {
+                mbar_arrive_expect_tx(&bars[C::kBarQ], 2u * C::kHalves * 64u * G * tpt * 2u);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                  uint8_t* q = smem + C::kOffQ + x * C::kQBytes;
+                  const int row = w.q_start + w.t0;
+#pragma unroll
+                  for (int hh = 0; hh < C::kHalves; ++hh)
+                    tma_load_3d(q + hh * kQHalf, &qmap, &bars[C::kBarQ], 64 * hh, w.h * G, row);
+                }
+              }
+            }
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            if (ok) ++n;
+          }
+        }
+      }
+      if (lane == 0) {
+        // Drain: the last Q and the last load issued into each stage have landed.
+        if (n > 0) (void)drain_wait(&bars[C::kBarQ], (n - 1) & 1);
+        for (int g = max(0, c - stages); g < c; ++g)
+          (void)drain_wait(&bars[bar_full + (g % stages)], (g / stages) & 1);
+      }
+    }
+  } else if (warp == kWarpTma) {
     // ------------------------------------------------------------ TMA producer
     // The whole warp walks the tiles so block ids arrive 32 at a time (one
     // coalesced load per 4 key tiles, shuffled to lane 0) instead of one L2
@@ -677,6 +792,47 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!(ok = wait_all(&bars[C::kBarKFull + kc % C::kKStages], (kc / C::kKStages) & 1))) break;
       tc_fence_after();
       const int nt = w.ntiles;
+      if constexpr (kShared) {
+        if (p.paired) {
+          // Tile A takes key tiles 2j of the unit, tile B 2j + 1. The order of the loads,
+          // K(0) K(1) V(0) K(2) V(1) ..., is the order they are used in here.
+          auto full = [&](int bar, int stages, int x) {
+            return wait_all(&bars[bar + x % stages], (x / stages) & 1);
+          };
+          auto free_k = [&](int x) {
+            if (leader) umma_commit(&bars[C::kBarKEmpty + x % C::kKStages]);
+          };
+          auto free_v = [&](int x) {
+            if (leader) umma_commit(&bars[C::kBarVEmpty + x % C::kVStages]);
+          };
+          for (int j = 0; j < nt; ++j) {
+            issue_s(0, kc + 2 * j);
+            free_k(kc + 2 * j);
+            if (j > 0) {
+              if (!(ok = full(C::kBarVFull, C::kVStages, vc + 2 * j - 1))) break;
+              if (!(ok = issue_pv(1, g + j - 1, vc + 2 * j - 1, j == 1, false))) break;
+              free_v(vc + 2 * j - 1);
+            }
+            if (!(ok = full(C::kBarKFull, C::kKStages, kc + 2 * j + 1))) break;
+            issue_s(1, kc + 2 * j + 1);
+            free_k(kc + 2 * j + 1);
+            if (leader && j + 1 == nt) umma_commit(&bars[C::kBarQFree]);
+            if (!(ok = full(C::kBarVFull, C::kVStages, vc + 2 * j))) break;
+            if (j + 1 < nt && !(ok = full(C::kBarKFull, C::kKStages, kc + 2 * j + 2))) break;
+            if (!(ok = issue_pv(0, g + j, vc + 2 * j, j == 0, j + 1 == nt))) break;
+            free_v(vc + 2 * j);
+          }
+          if (!ok) break;
+          if (!(ok = full(C::kBarVFull, C::kVStages, vc + 2 * nt - 1))) break;
+          if (!(ok = issue_pv(1, g + nt - 1, vc + 2 * nt - 1, nt == 1, true))) break;
+          free_v(vc + 2 * nt - 1);
+          kc += 2 * nt;
+          vc += 2 * nt;
+          g += nt;
+          ++n;
+          continue;
+        }
+      }
       for (int j = 0; j < nt; ++j) {
         issue_s(0, kc + j);
         if (j > 0) {
@@ -708,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (leader) umma_commit(&bars[C::kBarDone]);
     __syncwarp();
     (void)drain_wait(&bars[C::kBarDone], 0);
-  }  // warps 10 and 11 have no role
+  }  // warps 10 (unless paired) and 11 have no role
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ------------------------------------------------------------ softmax + epilogue
@@ -1034,7 +1190,8 @@ int launch_shared_prefix(const SharedPrefix& a, cudaStream_t s) {
   p.max_blocks = a.max_blocks;
   p.block_size = a.block_size;
   p.num_seqs = a.num_groups;
-  p.num_q_tiles = (a.max_group + 2 * tpt - 1) / (2 * tpt);
+  p.paired = a.paired;
+  p.num_q_tiles = a.paired ? 1 : (a.max_group + 2 * tpt - 1) / (2 * tpt);
   const int64_t items = static_cast<int64_t>(p.num_q_tiles) * a.num_kv_heads * a.num_groups;
   if (items * a.pieces >= (int64_t(1) << 31))
     return fail(PS_ERR_INVALID, "%s: too many query tiles for one launch", a.fn);

@@ -9,9 +9,12 @@ namespace ps {
 
 // Every row of group g (batch rows [group_starts[g], group_starts[g + 1])) attends
 // over keys [0, shared_lens[first row]) of its first row's block table, in
-// pieces of piece_keys keys (a multiple of 128). Piece x of batch row b and query
-// head h leaves its unnormalised output, running maximum (log2 units) and row sum
-// at row (x * num_seqs + b) * num_q_heads + h of part_o / part_ml.
+// pieces of piece_keys keys (a multiple of 128). Each piece leaves one partial result per
+// row (two when `paired`, for its even and odd key tiles): unnormalised output, running
+// maximum (log2 units) and row sum. Batch row b, KV head h and head g of its group is
+// row r = (h * num_seqs + b) * G + g of a partial; rows go in blocks of 32, a partial has
+// N = ceil(num_seqs * num_q_heads / 32) of them:
+//   part_o[partial][r / 32][column / 4][r % 32][column % 4]     part_ml[partial][r]
 struct SharedPrefix {
   const char* fn;
   const void* query;
@@ -33,6 +36,7 @@ struct SharedPrefix {
   int max_blocks;
   int pieces;
   int piece_keys;
+  bool paired;  // max_group rows fill one query tile at most
   float scale;
   float* part_o;
   float2* part_ml;

@@ -129,9 +129,10 @@ def test_nothing_shared_is_paged_decode():
     q = torch.randn((3, 8, 64), device=DEV).to(torch.float16)
     ref = ops.paged_decode(q, *pools, tables.to(DEV), _i32(lens), 0.125)
     assert torch.equal(_shared(q, pools, tables, lens, pre, starts), ref)
-    # a maximum that no row uses
+    # A maximum that no row uses: another instantiation runs, which promises the
+    # same attention, not the same bits.
     out = ops.paged_decode_shared(q, *pools, tables.to(DEV), _i32(lens), _i32(starts), _i32(pre), 3, 16, 0.125)
-    assert torch.equal(out, ref)
+    _check(out, q, pools, tables, lens, "nothing shared", HALF[torch.float16])
 
 
 def test_bad_lengths_are_reported():

@@ -148,11 +148,15 @@ def test_shared_refusals():
 def test_shared_workspace_and_pieces():
     size = ops.decode_shared_workspace_bytes
     one = size(4, 8, 128, 16, 8, 64, 0, 0)
-    assert one == 4 * 8 * 128 * 4 + 4 * 8 * 8
+    assert one == 2 * (4 * 8 * 128 * 4 + 4 * 8 * 8)  # two partials a piece
     assert size(4, 8, 128, 16, 80, 1280, 128, 0) == 10 * one
     assert size(4, 8, 128, 16, 8, 0, 0, 0) == 0
     assert size(4, 8, 128, 16, 8, 64, 0, 32) == one + ops.decode_workspace_bytes(4, 8, 128, 16, 8, 32)
-    # 256 rows x 4 heads = 4 pairs of tiles x 8 KV heads = 32 items over 8192 keys
-    keys = ops.shared_split_keys([256], 32, 8, 8192, 148)
-    assert keys % 128 == 0 and 32 * -(-8192 // keys) >= 0.8 * 148
+    # 256 rows x 4 heads = 4 pairs of tiles x 8 KV heads = 32 items: four pieces of 16 tiles
+    # are one wave of 128 units
+    assert ops.shared_split_keys([256], 32, 8, 8192, 148) == 2048
     assert ops.shared_split_keys([256], 32, 8, 128, 148) == 0
+    assert ops.shared_split_keys([], 32, 8, 8192, 148) == 0
+    for sizes, hq, hkv, keys in (([8], 64, 8, 32768), ([17, 3, 40], 14, 2, 2000), ([1], 8, 8, 64), ([500], 16, 1, 100000)):
+        split = ops.shared_split_keys(sizes, hq, hkv, keys, 148)
+        assert split % 128 == 0 and 0 <= split < keys
