@@ -147,6 +147,11 @@ __global__ void __launch_bounds__(NW * 32)
       if (b < 0) break;
     }
 
+    // The first block ids need not wait for the length: entries below max_blocks exist, and
+    // those past the context are dropped.
+    const int first_blk = split * p.part_tokens / BS;
+    const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride + first_blk;
+    const int32_t early = first_blk + static_cast<int>(threadIdx.x) < p.max_blocks ? bt[threadIdx.x] : 0;
     int ctx = p.ctx_lens[b];
     if (ctx > p.max_blocks * BS) {
       if (threadIdx.x == 0 && split == 0) set_device_error(p.err, PS_DEVERR_LENGTH);
@@ -166,9 +171,8 @@ __global__ void __launch_bounds__(NW * 32)
     const int n_keys = min(ctx - t_begin, p.part_tokens);
     const int nchunk = (n_keys + kKeys - 1) / kKeys;
     const int nblk = (n_keys + BS - 1) / BS;
-    const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride + t_begin / BS;
-    for (int i = threadIdx.x; i < nblk; i += blockDim.x) {
-      int32_t id = bt[i];
+    for (int i = threadIdx.x; i < nblk; i += NW * 32) {
+      int32_t id = i < NW * 32 ? early : bt[i];
       if (id < 0 || id >= p.num_blocks) {
         set_device_error(p.err, PS_DEVERR_BLOCK_ID);
         id = 0;  // read a valid block instead of faulting; the error bit reports it
@@ -519,6 +523,11 @@ __global__ void __launch_bounds__(NW * 32)
 // ------------------------------------------------------------ host side
 constexpr int kNW = 4;  // warps per CTA
 constexpr int kNS = 2;  // stages of 32 keys per warp
+// Warps per CTA of the unsplit launch: at head dim 64 a stage is half the bytes, and a CTA's
+// longest sequence sets the launch's length (96 sequences U[1,2000], Hq 14, Hkv 2, int8:
+// 16.9 against 19.2 us); at head dim 128 eight are slower (256 sequences: 247 against 199).
+template <int D>
+constexpr int unsplit_warps() { return D == 64 ? 8 : kNW; }
 
 template <typename T, typename C, int D, int BS, int R>
 int launch_quant(const QuantDecodeParams& qp, const CUtensorMap& km, const CUtensorMap& vm,
@@ -528,12 +537,14 @@ int launch_quant(const QuantDecodeParams& qp, const CUtensorMap& km, const CUten
   const size_t smem = SM::bytes(p.table_cap);
   const char* fn = "ps_paged_decode_quant";
   if (p.max_splits <= 1) {
-    auto kern = paged_decode_quant_kernel<T, C, D, kNW, kNS, BS, R, false>;
+    constexpr int NWU = unsplit_warps<D>();
+    auto kern = paged_decode_quant_kernel<T, C, D, NWU, kNS, BS, R, false>;
     static size_t configured[64] = {};
-    int st = reserve_smem(kern, smem, configured);
+    const size_t smem_u = QuantSmem<D, NWU, kNS>::bytes(p.table_cap);
+    int st = reserve_smem(kern, smem_u, configured);
     if (st != PS_OK) return st;
-    const cudaError_t e = launch_pdl(kern, dim3(p.num_kv_heads, 1, p.num_launch), dim3(kNW * 32),
-                                     smem, s, qp, km, vm);
+    const cudaError_t e = launch_pdl(kern, dim3(p.num_kv_heads, 1, p.num_launch), dim3(NWU * 32),
+                                     smem_u, s, qp, km, vm);
     if (e != cudaSuccess) return fail(PS_ERR_CUDA, "%s: launch failed: %s", fn, cudaGetErrorString(e));
     return check_launch(fn);
   }
