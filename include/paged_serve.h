@@ -532,7 +532,8 @@ PS_API int64_t ps_paged_decode_shared_workspace_bytes(int num_seqs, int num_q_he
  *
  * key/value/slot_mapping and strides as in ps_cache_append; dtype is the type of
  * key and value, code the pools' code type. Pools, scales, key and value must be
- * 16-byte aligned.
+ * 16-byte aligned. The slots of one call must be distinct (two rows for one slot may
+ * leave the codes of one with the scale of the other).
  */
 PS_API int ps_cache_append_quant(void* k_pool, void* v_pool, float* k_scale, float* v_scale,
                                  const void* key, const void* value, const int64_t* slot_mapping,
@@ -589,7 +590,7 @@ PS_API int ps_cache_read_quant(const void* k_pool, const void* v_pool, const flo
  * ps_paged_decode_listed (may be NULL with num_listed < 0); num_listed < 0 = all
  * num_seqs sequences, else the entries of seq_list to run; planned != 0 = the unit
  * list for these lengths, order and geometry is already in the workspace
- * (ps_paged_decode_plan), all sequences. Keys at or past ctx_lens[b] are not
+ * (ps_paged_decode_plan); it covers all sequences, so num_listed must be negative. Keys at or past ctx_lens[b] are not
  * used, whatever their rows and scales hold. Scores, softmax and accumulation are
  * float32; probabilities times V scales are rounded to fp16 for the second product.
  */

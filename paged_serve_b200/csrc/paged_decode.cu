@@ -802,7 +802,8 @@ int decode_entry(const char* fn, void* out, int64_t out_seq_stride, const void* 
     p.pre_ml = shared->part_ml;
     p.pre_keys = shared->piece_keys;
     p.pre_parts = shared->paired ? 2 : 1;
-    p.pre_max = shared->pieces * shared->piece_keys;
+    p.pre_max = static_cast<int>(
+        std::min<int64_t>(static_cast<int64_t>(shared->pieces) * shared->piece_keys, 0x7fffffff));
     return dispatch_decode<true>(p, km, vm, s, dtype, head_dim, block_size, shared);
   }
   return dispatch_decode<false>(p, km, vm, s, dtype, head_dim, block_size);
@@ -954,8 +955,10 @@ SharedLayout shared_layout(int num_seqs, int num_q_heads, int head_dim, int max_
                            int split_keys) {
   SharedLayout l;
   if (max_shared <= 0) return l;
-  l.piece_keys = split_keys > 0 ? split_keys : (max_shared + 127) / 128 * 128;
-  l.pieces = (max_shared + l.piece_keys - 1) / l.piece_keys;
+  const int64_t whole = (static_cast<int64_t>(max_shared) + 127) / 128 * 128;
+  l.piece_keys = static_cast<int>(split_keys > 0 ? std::min<int64_t>(split_keys, whole)
+                                                 : std::min<int64_t>(whole, 0x7fffff80));
+  l.pieces = static_cast<int>((static_cast<int64_t>(max_shared) + l.piece_keys - 1) / l.piece_keys);
   // Room for two partials a piece: whether a piece leaves one or two depends on the
   // groups' sizes, which the workspace should not.
   const int64_t rows = 2 * static_cast<int64_t>(l.pieces) *

@@ -620,6 +620,9 @@ extern "C" int ps_paged_decode_quant(
   if (num_listed > num_seqs || (num_listed > 0 && !seq_list))
     return fail(PS_ERR_INVALID, "%s: num_listed %d needs a list of at most num_seqs %d entries", fn,
                 num_listed, num_seqs);
+  if (planned && num_listed >= 0)
+    return fail(PS_ERR_INVALID, "%s: a plan covers all sequences; it cannot be combined with a list",
+                fn);
   if (num_listed == 0) return PS_OK;
   QuantDecodeParams qp{};
   DecodeParams& p = qp.d;

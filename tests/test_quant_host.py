@@ -65,11 +65,11 @@ def test_read_refusals():
 
 def _decode(**kw):
     a = dict(os=1024, qs=1024, ks=16, nb=8, bts=4, b=2, order=None, listed=-1, hq=8, hkv=2, d=128, bs=16, mb=4,
-             split=0, ws=None, wsb=0, dtype=2, code=1)
+             split=0, planned=0, ws=None, wsb=0, dtype=2, code=1)
     a.update(kw)
     return _lib.load().ps_paged_decode_quant(
         16, a["os"], 16, a["qs"], 16, 16, a["ks"], 16, a["nb"], 16, a["bts"], 16, a["b"], a["order"],
-        a["listed"], a["hq"], a["hkv"], a["d"], a["bs"], a["mb"], 0.1, a["split"], 0, a["ws"], a["wsb"],
+        a["listed"], a["hq"], a["hkv"], a["d"], a["bs"], a["mb"], 0.1, a["split"], a["planned"], a["ws"], a["wsb"],
         a["dtype"], a["code"], None, None)
 
 
@@ -85,6 +85,7 @@ def test_decode_refusals():
     assert _decode(listed=1) == _lib.PS_ERR_INVALID
     assert _decode(listed=3, order=16) == _lib.PS_ERR_INVALID
     assert _decode(listed=0) == _lib.PS_OK
+    assert _decode(listed=0, planned=1) == _lib.PS_ERR_INVALID and "plan" in _msg()
     assert _decode(b=0) == _lib.PS_OK
     assert _decode(split=24) == _lib.PS_ERR_INVALID
     assert _decode(split=16) == _lib.PS_ERR_INVALID and "workspace" in _msg()
@@ -151,6 +152,8 @@ def test_shared_workspace_and_pieces():
     assert one == 2 * (4 * 8 * 128 * 4 + 4 * 8 * 8)  # two partials a piece
     assert size(4, 8, 128, 16, 80, 1280, 128, 0) == 10 * one
     assert size(4, 8, 128, 16, 8, 0, 0, 0) == 0
+    assert size(4, 8, 128, 16, 8, 64, (1 << 31) - 128, 0) == one  # one piece, however long
+    assert size(4, 8, 128, 16, 8, 64, -128, 0) == 0 and size(4, 8, 128, 16, 8, -1, 0, 0) == 0
     assert size(4, 8, 128, 16, 8, 64, 0, 32) == one + ops.decode_workspace_bytes(4, 8, 128, 16, 8, 32)
     # 256 rows x 4 heads = 4 pairs of tiles x 8 KV heads = 32 items: four pieces of 16 tiles
     # are one wave of 128 units
