@@ -476,7 +476,8 @@ PS_API int64_t ps_paged_prefill_workspace_bytes(int num_seqs, int max_q_len, int
  *
  * Arguments as ps_paged_decode_ordered, and:
  * group_starts: [num_groups + 1] int32, group g = batch rows
- *   [group_starts[g], group_starts[g + 1]); at most max_group rows each.
+ *   [group_starts[g], group_starts[g + 1]); at most max_group rows each (groups that
+   share nothing may be longer).
  * shared_lens: [num_seqs] int32, the shared keys of each row: a multiple of
  *   block_size, at most ctx_lens[b] and max_shared, the same for all rows of a
  *   group, 0 for a row that shares nothing (such rows need no group; every row with

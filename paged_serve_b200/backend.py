@@ -35,6 +35,12 @@ A third entry, :meth:`PagedCudaBackend.begin_plan`, takes a
 copy-on-write): one pinned upload of the tables and lengths, one launch of the
 copy-on-write block copies over all layers, one launch that builds the slots
 and positions on the device.
+
+Two options change what a step reads. ``kv_codes`` holds the cache in 8 bits
+(:func:`ops.cache_append_quant`): decode steps attend over the codes, prefill steps over
+the sequences' tokens read back to 16 bits. ``share_prefixes`` lets a block-manager
+decode step read leading blocks that neighbouring sequences share once for all of them
+(:func:`ops.paged_decode_shared`).
 """
 
 from __future__ import annotations
@@ -88,6 +94,18 @@ class PagedMetadata(AttentionMetadata):
     # Prefill steps with few query tiles over long contexts: keys per split-K
     # piece (ops.prefill_split_keys; 0 = items run whole).
     prefill_split_keys: int = 0
+    # 8-bit cache, steps that prefill: where each prefilling sequence's tokens are read
+    # back to (int32 [B, W] blocks of the 16-bit scratch pool) and how many (int32 [B],
+    # 0 for the others).
+    read_tables: torch.Tensor | None = None
+    read_lens: torch.Tensor | None = None
+    # Decode steps whose neighbours share leading blocks: int32 [groups + 1] first rows,
+    # int32 [B] shared tokens, the largest of each, and the keys per piece.
+    group_starts: torch.Tensor | None = None
+    shared_lens: torch.Tensor | None = None
+    max_group: int = 0
+    max_shared: int = 0
+    shared_split_keys: int = 0
 
 
 class PagedCudaBackend(AttentionBackend):
@@ -109,6 +127,8 @@ class PagedCudaBackend(AttentionBackend):
         split_mixed_steps: bool = True,
         overlap_mixed_steps: bool = True,
         split_prefill: bool = True,
+        kv_codes: torch.dtype | None = None,
+        share_prefixes: bool = False,
     ) -> None:
         """
         Args:
@@ -139,6 +159,14 @@ class PagedCudaBackend(AttentionBackend):
                 CTAs and merged by a second launch (a long prompt's chunk over
                 its long cached prefix); mixed steps hide their prefill under the
                 decode instead and never split it.
+            kv_codes: ``torch.float8_e4m3fn`` or ``torch.int8`` holds the cache in 8
+                bits with a float32 scale per (token, KV head) row; None in ``dtype``.
+                A prefilling sequence's tokens are read back into a 16-bit scratch
+                pool of its own length, shared by the layers.
+            share_prefixes: a decode step planned by the block manager reads leading
+                blocks that neighbouring sequences of the plan share once for the
+                group, where that saves enough keys (:func:`shared_groups`); not with
+                ``kv_codes``. Schedule sequences of one prompt next to each other.
         """
         if model.num_q_heads % model.num_kv_heads != 0:
             raise ValueError("num_q_heads must be divisible by num_kv_heads")
@@ -154,6 +182,18 @@ class PagedCudaBackend(AttentionBackend):
         self.overlap_mixed_steps = overlap_mixed_steps
         self._side_stream: torch.cuda.Stream | None = None
         self.split_prefill = split_prefill
+        if kv_codes is not None and kv_codes not in ops.CODES:
+            raise ValueError(f"kv_codes must be float8_e4m3fn or int8, not {kv_codes}")
+        if kv_codes is not None and share_prefixes:
+            raise ValueError("share_prefixes reads 16-bit pools; it cannot be combined with kv_codes")
+        self.kv_codes = kv_codes
+        self.share_prefixes = share_prefixes
+        self.k_scale: torch.Tensor | None = None  # [L, num_blocks, Hkv, bs] with kv_codes
+        self.v_scale: torch.Tensor | None = None
+        self.host_k_scale: torch.Tensor | None = None
+        self.host_v_scale: torch.Tensor | None = None
+        self._scratch: tuple[torch.Tensor, torch.Tensor] | None = None  # read-back pools
+        self._shared_ws: torch.Tensor | None = None
         self._prefill_ws: torch.Tensor | None = None  # split-K prefill partials, grown on demand
         self._num_sms = 0
         self.scale = 1.0 / math.sqrt(model.head_dim)
@@ -188,8 +228,15 @@ class PagedCudaBackend(AttentionBackend):
         self.max_blocks_per_seq = math.ceil(max_seq_len / bs)
         self.num_blocks = self.requested_blocks or num_seq_slots * self.max_blocks_per_seq
         shape = (m.num_layers, self.num_blocks, m.num_kv_heads, bs, m.head_dim)
-        self.k_cache = torch.zeros(shape, device=self.device, dtype=self.dtype)
-        self.v_cache = torch.zeros(shape, device=self.device, dtype=self.dtype)
+        if self.kv_codes is None:
+            self.k_cache = torch.zeros(shape, device=self.device, dtype=self.dtype)
+            self.v_cache = torch.zeros(shape, device=self.device, dtype=self.dtype)
+        else:
+            self.k_cache, self.v_cache = (
+                torch.zeros(shape, device=self.device, dtype=torch.uint8).view(self.kv_codes)
+                for _ in range(2))
+            self.k_scale, self.v_scale = (
+                torch.zeros(shape[:-1], device=self.device, dtype=torch.float32) for _ in range(2))
         if num_seq_slots * self.max_blocks_per_seq <= self.num_blocks:
             self._identity_tables = torch.arange(
                 num_seq_slots * self.max_blocks_per_seq, device=self.device, dtype=torch.int32
@@ -216,14 +263,21 @@ class PagedCudaBackend(AttentionBackend):
         if self.k_cache is None:
             raise RuntimeError("allocate() must be called before allocate_swap_space()")
         shape = (self.k_cache.shape[0], num_host_blocks) + tuple(self.k_cache.shape[2:])
-        self.host_k_cache = torch.empty(shape, dtype=self.dtype, pin_memory=True)
-        self.host_v_cache = torch.empty(shape, dtype=self.dtype, pin_memory=True)
+        dtype = self.kv_codes or self.dtype
+        self.host_k_cache = torch.empty(shape, dtype=dtype, pin_memory=True)
+        self.host_v_cache = torch.empty(shape, dtype=dtype, pin_memory=True)
+        if self.kv_codes is not None:
+            self.host_k_scale = torch.empty(shape[:-1], pin_memory=True)
+            self.host_v_scale = torch.empty(shape[:-1], pin_memory=True)
 
     def free(self) -> None:
         self._static = {}
         self._manager = None
         self.host_k_cache = None
         self.host_v_cache = None
+        self.k_scale = self.v_scale = self.host_k_scale = self.host_v_scale = None
+        self._scratch = None
+        self._shared_ws = None
         self.k_cache = None
         self.v_cache = None
         self._identity_tables = None
@@ -293,9 +347,29 @@ class PagedCudaBackend(AttentionBackend):
             keys = self._plan_prefill_split(self._prefill_items(None, b, tq), tq, b, key_len)
             if keys:
                 md = dataclasses.replace(md, prefill_split_keys=keys)
+        if self.kv_codes is not None and tq > 1:
+            w = -(-key_len // bs)
+            rows = torch.arange(b * w, dtype=torch.int32, device=dev).view(b, w)
+            md = self._plan_read(md, rows, ctx_lens, b * w)
         if self.debug_invariants:
             self._validate(md)
         return md
+
+    def _plan_read(self, md: PagedMetadata, tables: torch.Tensor, lens: torch.Tensor,
+                   blocks: int) -> PagedMetadata:
+        """Metadata with the step's read-back ([B, W] scratch blocks, tokens per sequence),
+        and a scratch pool of at least ``blocks`` blocks."""
+        m = self.model
+        if self._scratch is None or self._scratch[0].shape[0] < blocks:
+            shape = (blocks, m.num_kv_heads, self.block_size, m.head_dim)
+            self._scratch = tuple(torch.empty(shape, device=self.device, dtype=self.dtype)
+                                  for _ in range(2))
+        # Source and destination tables of one width (the source's may be wider or narrower).
+        w = tables.shape[1]
+        src = md.block_tables
+        if src.shape[1] < w:
+            tables = tables[:, : src.shape[1]].contiguous()
+        return dataclasses.replace(md, read_tables=tables, read_lens=lens.contiguous())
 
     def _decode_order(self, ctx_lens: torch.Tensor, query_len: int) -> torch.Tensor | None:
         """Longest-first order for the step's decode launches (one launch per step)."""
@@ -357,22 +431,38 @@ class PagedCudaBackend(AttentionBackend):
         return torch.tensor(pairs, dtype=torch.int64).pin_memory().to(self.device,
                                                                       non_blocking=True)
 
+    def _pools(self, host: bool = False) -> list[tuple[torch.Tensor, torch.Tensor]]:
+        """The (K, V) pools a block move covers: the cache, and its scales if it has any
+        (as blocks of one-element rows)."""
+        if host:
+            pools = [(self.host_k_cache, self.host_v_cache)]
+            scales = (self.host_k_scale, self.host_v_scale)
+        else:
+            pools = [(self.k_cache, self.v_cache)]
+            scales = (self.k_scale, self.v_scale)
+        if scales[0] is not None:
+            pools.append((scales[0].unsqueeze(-1), scales[1].unsqueeze(-1)))
+        return pools
+
     def apply_block_moves(self, plan: StepPlan) -> None:
         """Run a plan's swap-outs, then swap-ins, then copy-on-write copies."""
         if plan.swap_out or plan.swap_in:
             if self.host_k_cache is None:
                 raise RuntimeError("the plan moves blocks but no swap space is allocated")
         if plan.swap_out:
-            ops.swap_blocks(self.host_k_cache, self.host_v_cache, self.k_cache, self.v_cache,
-                            self._pairs(plan.swap_out), self.swap_max_ctas, self.device_error)
+            pairs = self._pairs(plan.swap_out)
+            for dst, src in zip(self._pools(host=True), self._pools()):
+                ops.swap_blocks(*dst, *src, pairs, self.swap_max_ctas, self.device_error)
         if plan.swap_in:
-            ops.swap_blocks(self.k_cache, self.v_cache, self.host_k_cache, self.host_v_cache,
-                            self._pairs(plan.swap_in), self.swap_max_ctas, self.device_error)
+            pairs = self._pairs(plan.swap_in)
+            for dst, src in zip(self._pools(), self._pools(host=True)):
+                ops.swap_blocks(*dst, *src, pairs, self.swap_max_ctas, self.device_error)
         if plan.copies:
             if self.debug_invariants:
                 ops.check_block_pairs(plan.copies)
-            ops.copy_blocks(self.k_cache, self.v_cache, self._pairs(plan.copies),
-                            self.device_error)
+            pairs = self._pairs(plan.copies)
+            for k, v in self._pools():
+                ops.copy_blocks(k, v, pairs, self.device_error)
 
     def begin_plan(self, plan: StepPlan, width: int | None = None) -> PagedMetadata | None:
         """Device metadata for a block-manager step, after running its block moves.
@@ -410,6 +500,24 @@ class PagedCudaBackend(AttentionBackend):
                    + [i * tq + tq - n for i, n in enumerate(plan.q_lens)])
         if dec:
             buf.extend([0 if n == 1 else n for n in plan.q_lens] + dec)
+        extra = len(buf)
+        read_w = read_blocks = 0
+        groups = None
+        if self.kv_codes is not None and tq > 1:
+            # Scratch blocks of the sequences the prefill kernel attends, one after another.
+            pre = [0 if n == 0 or (n == 1 and dec) else x for n, x in zip(plan.q_lens, lens)]
+            read_w = max(-(-x // self.block_size) for x in pre)
+            rows = array("i", bytes(4 * b * read_w))
+            for i, x in enumerate(pre):
+                n = -(-x // self.block_size)
+                rows[i * read_w : i * read_w + n] = array("i", range(read_blocks, read_blocks + n))
+                read_blocks += n
+            buf.extend(rows)
+            buf.extend(pre)
+        elif self.share_prefixes and tq == 1 and dev.type == "cuda":
+            groups = shared_groups(plan.tables, lens, self.block_size, self._min_shared_keys())
+            if groups is not None:
+                buf.extend(groups[0] + groups[1])
         host = torch.frombuffer(buf, dtype=torch.int32)
         if dev.type == "cuda":
             host = host.pin_memory()
@@ -419,7 +527,7 @@ class PagedCudaBackend(AttentionBackend):
         decode_list = prefill_q_lens = None
         if dec:
             prefill_q_lens = packed[b * w + 4 * b : b * w + 5 * b]
-            decode_list = packed[b * w + 5 * b :]
+            decode_list = packed[b * w + 5 * b : extra]
         slots, positions = ops.build_slot_mapping(tables, ctx_before, q_lens, tq, self.block_size,
                                                   self.num_blocks, True, self.device_error)
         live = torch.tensor(sum(lens), dtype=torch.int64)
@@ -432,17 +540,48 @@ class PagedCudaBackend(AttentionBackend):
             num_prefill_seqs=sum(1 for n in plan.q_lens if n > 1),
         )
         self._live_tokens = live
-        if self._plan_decode(md):
+        if groups is None and self._plan_decode(md):
             md = dataclasses.replace(md, decode_planned=True)
         elif tq > 1 and not dec:
             keys = self._plan_prefill_split(self._prefill_items(plan.q_lens, b, tq), tq, b,
                                             max(lens))
             if keys:
                 md = dataclasses.replace(md, prefill_split_keys=keys)
+        if read_w:
+            md = self._plan_read(md, packed[extra : extra + b * read_w].view(b, read_w),
+                                 packed[extra + b * read_w :], read_blocks)
+        elif groups is not None:
+            md = self._plan_shared(md, groups, packed[extra : extra + len(groups[0])],
+                                   packed[extra + len(groups[0]) :])
         if self.debug_invariants:
             self._validate(md)
             self._check_device_error()
         return md
+
+    def _min_shared_keys(self) -> int:
+        """Keys a shared-prefix decode must save a layer to be worth its prefix pass."""
+        m = self.model
+        return SHARED_MIN_VALUES // (m.num_kv_heads * m.head_dim)
+
+    def _plan_shared(self, md: PagedMetadata, groups, starts: torch.Tensor,
+                     shared: torch.Tensor) -> PagedMetadata:
+        m = self.model
+        if not self._num_sms:
+            self._num_sms = torch.cuda.get_device_properties(self.device).multi_processor_count
+        first, pre = groups
+        sizes = [z - a for a, z in zip(first, first[1:]) if pre[a]]
+        max_shared = max(pre)
+        keys = ops.shared_split_keys(sizes, m.num_q_heads, m.num_kv_heads, max_shared,
+                                     self._num_sms)
+        need = ops.decode_shared_workspace_bytes(
+            md.num_seqs, m.num_q_heads, m.head_dim, self.block_size, md.block_tables.shape[1],
+            max_shared, keys, self.split_tokens)
+        if self._shared_ws is None or self._shared_ws.numel() < need:
+            self._shared_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return dataclasses.replace(
+            md, group_starts=starts, shared_lens=shared, max_group=max(sizes),
+            max_shared=max_shared, shared_split_keys=keys,
+            seq_order=ops.decode_order(md.ctx_lens - shared))
 
     # ------------------------------------------------------------------ CUDA graphs
     def static_decode_metadata(self, batch: int, width: int | None = None) -> PagedMetadata:
@@ -605,12 +744,23 @@ class PagedCudaBackend(AttentionBackend):
         hkv = self.model.num_kv_heads
         k_pool = self.k_cache[layer_idx]
         v_pool = self.v_cache[layer_idx]
-        if tq == 1:
+        if self.kv_codes is not None:
+            out = self._forward_quant(layer_idx, query, key, value, md)
+        elif md.group_starts is not None:
+            # Shared prefixes: append, then the prefix pass and the decode behind it.
+            ops.cache_append(k_pool, v_pool, key.reshape(b, hkv, d), value.reshape(b, hkv, d),
+                             md.slot_mapping, self.device_error)
+            out = ops.paged_decode_shared(
+                query.reshape(b, hq, d), k_pool, v_pool, md.block_tables, md.ctx_lens,
+                md.group_starts, md.shared_lens, md.max_group, md.max_shared, self.scale,
+                split_keys=md.shared_split_keys, split_tokens=self.split_tokens,
+                out=self._out_buffer(layer_idx, b), workspace=self._shared_ws,
+                device_error=self.device_error, seq_order=md.seq_order,
+            ).view(b, 1, hq, d)
+        elif tq == 1:
             # One launch: each sequence's new K/V row is written by the CTA that
             # then attends over it (same pool contents as append + decode).
-            buf = None
-            if self._decode_out is not None and b <= self._decode_out.shape[1]:
-                buf = self._decode_out[layer_idx, :b]
+            buf = self._out_buffer(layer_idx, b)
             out = ops.paged_decode_append(
                 query.reshape(b, hq, d), key.reshape(b, hkv, d), value.reshape(b, hkv, d),
                 md.slot_mapping, k_pool, v_pool, md.block_tables, md.ctx_lens,
@@ -674,6 +824,49 @@ class PagedCudaBackend(AttentionBackend):
             self._check_device_error()
         return out
 
+    def _out_buffer(self, layer_idx: int, batch: int) -> torch.Tensor | None:
+        """The layer's decode output buffer, None for a batch larger than it."""
+        if self._decode_out is not None and batch <= self._decode_out.shape[1]:
+            return self._decode_out[layer_idx, :batch]
+        return None
+
+    def _forward_quant(self, layer_idx: int, query, key, value, md: PagedMetadata) -> torch.Tensor:
+        """forward() over an 8-bit cache: quantise the step's tokens into it, then decode from
+        the codes and prefill from the sequences' tokens read back to 16 bits."""
+        b, tq, hq, d = query.shape
+        hkv = self.model.num_kv_heads
+        cache = (self.k_cache[layer_idx], self.v_cache[layer_idx], self.k_scale[layer_idx],
+                 self.v_scale[layer_idx])
+        err = self.device_error
+        ops.cache_append_quant(*cache, key.reshape(b * tq, hkv, d), value.reshape(b * tq, hkv, d),
+                               md.slot_mapping, err)
+        if tq == 1:
+            return ops.paged_decode_quant(
+                query.reshape(b, hq, d), *cache, md.block_tables, md.ctx_lens, self.scale,
+                self.split_tokens, out=self._out_buffer(layer_idx, b), workspace=self._workspace,
+                device_error=err, seq_order=md.seq_order, planned=md.decode_planned,
+            ).view(b, 1, hq, d)
+        flat = query.reshape(b * tq, hq, d)
+        out = torch.empty_like(flat)
+        q_lens = md.q_lens
+        if md.decode_list is not None:
+            q_lens = md.prefill_q_lens
+            ops.paged_decode_quant(
+                flat.view(b, tq, hq, d)[:, tq - 1], *cache, md.block_tables, md.ctx_lens,
+                self.scale, self.split_tokens, out=out.view(b, tq, hq, d)[:, tq - 1],
+                workspace=self._workspace, device_error=err, seq_list=md.decode_list)
+        if md.decode_list is None or md.num_prefill_seqs:
+            k, v = self._scratch
+            w = md.read_tables.shape[1]
+            ops.cache_read_quant(*cache, md.block_tables[:, :w], md.read_lens, k, v,
+                                 md.read_tables, err)
+            split = md.prefill_split_keys
+            ops.paged_prefill(flat, k, v, md.read_tables, md.q_starts, q_lens, md.ctx_before, tq,
+                              self.scale, out=out, device_error=err, split_keys=split,
+                              workspace=self._prefill_ws if split else None,
+                              max_keys=md.key_len)
+        return out.view(b, tq, hq, d)
+
     def write_kv_rope(
         self, layer_idx: int, key: torch.Tensor, value: torch.Tensor, metadata: PagedMetadata
     ) -> None:
@@ -691,6 +884,13 @@ class PagedCudaBackend(AttentionBackend):
             self._rope_table = cos_sin_table(self.model.head_dim, theta, self.max_seq_len,
                                              self.dtype, self.device)
         b, tq, hkv, d = key.shape
+        if self.kv_codes is not None:
+            ops.cache_append_rope_quant(
+                self.k_cache[layer_idx], self.v_cache[layer_idx], self.k_scale[layer_idx],
+                self.v_scale[layer_idx], key.reshape(b * tq, hkv, d),
+                value.reshape(b * tq, hkv, d), metadata.slot_mapping, metadata.positions,
+                self._rope_table, self.device_error)
+            return
         ops.cache_append_rope(self.k_cache[layer_idx], self.v_cache[layer_idx],
                               key.reshape(b * tq, hkv, d), value.reshape(b * tq, hkv, d),
                               metadata.slot_mapping, metadata.positions, self._rope_table,
@@ -711,7 +911,9 @@ class PagedCudaBackend(AttentionBackend):
         if self.k_cache is None:
             return KVMemoryStats(allocated_bytes=0, live_bytes=0)
         per_token = self._kv_bytes_per_token()
-        allocated = 2 * self.k_cache.numel() * self.k_cache.element_size()
+        allocated = 2 * self.k_cache.nbytes
+        if self.k_scale is not None:
+            allocated += 2 * self.k_scale.nbytes
         if self._manager is not None:
             return KVMemoryStats(allocated_bytes=allocated,
                                  live_bytes=self._manager.physical_tokens() * per_token)
@@ -728,7 +930,47 @@ class PagedCudaBackend(AttentionBackend):
 
     def _kv_bytes_per_token(self) -> int:
         m = self.model
-        return 2 * m.num_layers * m.num_kv_heads * m.head_dim * self.k_cache.element_size()
+        row = m.head_dim * self.k_cache.element_size() + (4 if self.k_scale is not None else 0)
+        return 2 * m.num_layers * m.num_kv_heads * row
+
+
+# Values (keys x KV heads x head dim) a shared-prefix decode must not have to read again
+# before it replaces the plain decode.
+SHARED_MIN_VALUES = 1 << 24
+
+
+def shared_groups(tables, lens, block_size: int, min_saved: int):
+    """Groups of neighbouring sequences that share leading blocks.
+
+    ``tables``: each sequence's block ids; ``lens``: its tokens, the newest included.
+    Returns (first rows ``[groups + 1]``, shared tokens per sequence ``[B]``), every row in one
+    group, or None when all groups together save fewer than ``min_saved`` keys. A group
+    grows while that saves more keys ((rows - 1) x shared tokens), and only whole blocks
+    behind which every row has a token of its own are shared.
+    """
+    first, pre = [0], []
+    saved = 0
+    n = len(tables)
+    i = 0
+    while i < n:
+        head = tables[i]
+        common = min(len(head), max(lens[i] - 1, 0) // block_size)
+        j = i + 1
+        while j < n:
+            limit = min(common, len(tables[j]), max(lens[j] - 1, 0) // block_size)
+            c = 0
+            while c < limit and tables[j][c] == head[c]:
+                c += 1
+            if c == 0 or (j - i) * c < (j - i - 1) * common:
+                break
+            common = c
+            j += 1
+        shared = common * block_size if j - i > 1 else 0
+        saved += (j - i - 1) * shared
+        pre += [shared] * (j - i)
+        first.append(j)
+        i = j
+    return (first, pre) if saved >= max(min_saved, 1) else None
 
 def native_library_loaded() -> bool:
     """True once the C-ABI library has been loaded into this process."""

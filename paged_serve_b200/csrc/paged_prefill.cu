@@ -186,16 +186,16 @@ __device__ __forceinline__ bool decode_item(const PrefillParams& p, int u, Item&
     w.q_start = p.q_starts[w.b];
     w.q_len = p.q_starts[w.b + 1] - w.q_start;
     if (w.t0 >= w.q_len) return false;
-    if (w.q_start < 0 || w.q_len > p.num_rows - w.q_start ||
-        w.q_len > nq * (p.paired ? 1 : 2) * p.tokens_per_tile) {
+    if (w.q_start < 0 || w.q_len > p.num_rows - w.q_start) {
       if (report) set_device_error(p.err, PS_DEVERR_LENGTH);
       return false;
     }
     w.ctx = p.ctx_lens[w.q_start];
+    if (w.ctx == 0) return false;  // nothing shared
     const int64_t room = static_cast<int64_t>(p.splits) * p.split_tiles * kN;  // pieces' keys
-    if (w.ctx <= 0 || w.ctx > p.max_blocks * p.block_size || w.ctx > room ||
-        w.ctx % p.block_size != 0) {
-      if (report && w.ctx != 0) set_device_error(p.err, PS_DEVERR_LENGTH);
+    if (w.ctx < 0 || w.ctx > p.max_blocks * p.block_size || w.ctx > room ||
+        w.ctx % p.block_size != 0 || w.q_len > nq * (p.paired ? 1 : 2) * p.tokens_per_tile) {
+      if (report) set_device_error(p.err, PS_DEVERR_LENGTH);
       return false;
     }
     const int item_tiles = (w.ctx + kN - 1) / kN;
