@@ -106,6 +106,7 @@ class PagedMetadata(AttentionMetadata):
     max_group: int = 0
     max_shared: int = 0
     shared_split_keys: int = 0
+    shared_split_tokens: int = 0  # split-K of the keys behind the prefixes, where any needs it
 
 
 class PagedCudaBackend(AttentionBackend):
@@ -551,7 +552,7 @@ class PagedCudaBackend(AttentionBackend):
             md = self._plan_read(md, packed[extra : extra + b * read_w].view(b, read_w),
                                  packed[extra + b * read_w :], read_blocks)
         elif groups is not None:
-            md = self._plan_shared(md, groups, packed[extra : extra + len(groups[0])],
+            md = self._plan_shared(md, groups, lens, packed[extra : extra + len(groups[0])],
                                    packed[extra + len(groups[0]) :])
         if self.debug_invariants:
             self._validate(md)
@@ -563,7 +564,7 @@ class PagedCudaBackend(AttentionBackend):
         m = self.model
         return SHARED_MIN_VALUES // (m.num_kv_heads * m.head_dim)
 
-    def _plan_shared(self, md: PagedMetadata, groups, starts: torch.Tensor,
+    def _plan_shared(self, md: PagedMetadata, groups, lens: list[int], starts: torch.Tensor,
                      shared: torch.Tensor) -> PagedMetadata:
         m = self.model
         if not self._num_sms:
@@ -571,16 +572,21 @@ class PagedCudaBackend(AttentionBackend):
         first, pre = groups
         sizes = [z - a for a, z in zip(first, first[1:]) if pre[a]]
         max_shared = max(pre)
+        # Short keys behind the prefixes need no split-K (two launches less); an unsplit
+        # launch stages a whole table row, so wide tables keep it.
+        split = self.split_tokens
+        if max(n - p for n, p in zip(lens, pre)) <= split and md.block_tables.shape[1] <= 4096:
+            split = 0
         keys = ops.shared_split_keys(sizes, m.num_q_heads, m.num_kv_heads, max_shared,
                                      self._num_sms)
         need = ops.decode_shared_workspace_bytes(
             md.num_seqs, m.num_q_heads, m.head_dim, self.block_size, md.block_tables.shape[1],
-            max_shared, keys, self.split_tokens)
+            max_shared, keys, split)
         if self._shared_ws is None or self._shared_ws.numel() < need:
             self._shared_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         return dataclasses.replace(
             md, group_starts=starts, shared_lens=shared, max_group=max(sizes),
-            max_shared=max_shared, shared_split_keys=keys,
+            max_shared=max_shared, shared_split_keys=keys, shared_split_tokens=split,
             seq_order=ops.decode_order(md.ctx_lens - shared))
 
     # ------------------------------------------------------------------ CUDA graphs
@@ -753,7 +759,7 @@ class PagedCudaBackend(AttentionBackend):
             out = ops.paged_decode_shared(
                 query.reshape(b, hq, d), k_pool, v_pool, md.block_tables, md.ctx_lens,
                 md.group_starts, md.shared_lens, md.max_group, md.max_shared, self.scale,
-                split_keys=md.shared_split_keys, split_tokens=self.split_tokens,
+                split_keys=md.shared_split_keys, split_tokens=md.shared_split_tokens,
                 out=self._out_buffer(layer_idx, b), workspace=self._shared_ws,
                 device_error=self.device_error, seq_order=md.seq_order,
             ).view(b, 1, hq, d)
@@ -934,9 +940,13 @@ class PagedCudaBackend(AttentionBackend):
         return 2 * m.num_layers * m.num_kv_heads * row
 
 
-# Values (keys x KV heads x head dim) a shared-prefix decode must not have to read again
-# before it replaces the plain decode.
-SHARED_MIN_VALUES = 1 << 24
+# K (or V) values a shared-prefix decode must save a layer before it replaces the plain decode:
+# saved keys x KV heads x head dim. Its prefix pass costs about 7 to 15 us of launches and
+# lookups, what reading these takes. One group, a layer's append and decode, plain against
+# shared: Hq 32, Hkv 8, D 128, 16 rows over 1024 keys (15 M values) 21.5 / 24.6 us, 4 over
+# 16384 (48 M) 41.0 / 37.4, 64 over 4096 (252 M) 108.6 / 39.9; Hq 14, Hkv 2, D 64, 64 over
+# 1024 (8 M) 15.4 / 20.5, 64 over 4096 (31 M) 25.1 / 24.1.
+SHARED_MIN_VALUES = 1 << 25
 
 
 def shared_groups(tables, lens, block_size: int, min_saved: int):

@@ -28,6 +28,18 @@
 //   O^T[16 dims x 8 heads] += V^T[16 x 16 keys] . P^T
 // The K codes of four neighbouring dims reach a lane as one 32-bit register; which
 // of the MMA's k indices they stand for is free as long as Q is laid out alike.
+//
+// Bound by HBM, with half the bytes of the 16-bit cache to hide the same work behind:
+// 256 sequences U[512,4096], Hq 32, Hkv 8, D 128, e4m3, blocks of 16 take 191-196 us by
+// box for 1.293 GB (6,600-6,750 GB/s, 1.02-1.04 of the copy peak; the 16-bit cache takes
+// 347 us). A warp spends 1,200-1,500 cycles on a stage of 32 keys and about 800 on
+// issuing the next one; twelve warps per SM hide both. Measured and not kept: 2 to 16
+// warps of 1 to 4 stages and stages of 16 keys (193 to 324 us); a producer warp per CTA
+// feeding four others through a shared ring (870 cycles to issue a stage: 226 us with
+// TMA, 202 us with 16-byte asynchronous copies); persistent CTAs taking over pending
+// ones with the next unit's keys prefetched during the merge (no gain: the other CTAs of
+// an SM cover a CTA's start). Partitions of 512 keys (64 sequences lognormal to 32768, Hq
+// 64) take 78 us for 338 MB: a unit's lookup, queries and merge are a third of its time.
 #include <cudaTypedefs.h>
 
 #include "decode_common.cuh"
@@ -58,7 +70,7 @@ struct QuantSmem {
   }
   // Byte offset of 16-byte chunk c of key t inside a swizzled tile: a row of 128
   // bytes spreads over 8 rows (128-byte swizzle), one of 64 bytes over 4 pairs of
-  // rows (64-byte swizzle); ldmatrix's 8 rows then hit 8 different banks groups.
+  // rows (64-byte swizzle); ldmatrix's 8 rows then hit 8 different groups of banks.
   __device__ __forceinline__ static uint32_t off(int t, int c) {
     return D == 128 ? t * 128 + ((c ^ (t & 7)) << 4) : t * 64 + ((c ^ ((t >> 1) & 3)) << 4);
   }

@@ -34,6 +34,14 @@
 // Barrier phases: every barrier completes at most once per key tile, and each
 // waiter is at most one phase behind (S_X(j+1) needs P_X(j), which needs the
 // softmax to have seen S_X(j)), so parity waits never alias.
+// kShared: the shared-prefix pass of a decode step (shared_prefix.h). The query rows
+// are the batch rows of a group, every key tile is a full one (no causal mask) and
+// every unit leaves partials. 256 rows of 4 heads over 8192 keys, 8 KV heads, D 128 (34
+// GFLOP): 43 us of this kernel under ncu's cold caches in four pieces, 0.47 of the
+// burst peak, bound by the per-tile chain and, with 16 key tiles a unit, by a unit's
+// start and end (about five key tiles' time). 8 rows of 8 heads over 32768 keys (134 MB):
+// 36 us in 16 pieces of paired tiles, 0.57 of the copy peak.
+//
 // All waits are bounded; a timeout sets PS_DEVERR_TIMEOUT and a shared abort
 // flag so every role leaves its loop, drains its in-flight copies / MMAs and
 // frees TMEM before the CTA exits.
