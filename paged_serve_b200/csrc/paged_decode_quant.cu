@@ -20,7 +20,7 @@
 //
 // Work decomposition as in paged_decode.cu: one CTA per (KV head, sequence), or
 // persistent CTAs claiming (KV head, partition) units; each warp owns a ring of
-// stages of 32 keys filled by TMA (codes) and bulk copies (scales). The group of
+// stages of 32 keys filled by TMA (codes) and 16-byte asynchronous copies (scales). The group of
 // query heads is the N side of the MMAs and the keys (for S) or the dims (for O)
 // the M side, so eight heads fill a tile that would be half padding the other
 // way round:
@@ -30,8 +30,8 @@
 // of the MMA's k indices they stand for is free as long as Q is laid out alike.
 //
 // Bound by HBM, with half the bytes of the 16-bit cache to hide the same work behind:
-// 256 sequences U[512,4096], Hq 32, Hkv 8, D 128, e4m3, blocks of 16 take 191-196 us by
-// box for 1.293 GB (6,600-6,750 GB/s, 1.02-1.04 of the copy peak; the 16-bit cache takes
+// 256 sequences U[512,4096], Hq 32, Hkv 8, D 128, e4m3, blocks of 16 take 191-209 us by
+// box for 1.293 GB (6,190-6,790 GB/s, 0.96-1.05 of the copy peak; the 16-bit cache takes
 // 347 us). A warp spends 1,200-1,500 cycles on a stage of 32 keys and about 800 on
 // issuing the next one; twelve warps per SM hide both. Measured and not kept: 2 to 16
 // warps of 1 to 4 stages and stages of 16 keys (193 to 324 us); a producer warp per CTA
@@ -61,7 +61,6 @@ struct QuantSmem {
   static constexpr int kTileBytes = kKeys * D;  // K or V codes of one stage
   static constexpr int kRingBytes = NW * NS * 2 * kTileBytes;
   static constexpr int kScaleOffset = kRingBytes;  // per stage: 32 K scales, 32 V scales
-  static constexpr int kStageTx = 2 * kTileBytes + 2 * kKeys * 4;
   static constexpr int kBarOffset = kScaleOffset + NW * NS * 2 * kKeys * 4;
   static constexpr int kTableOffset = kBarOffset + NW * NS * 8;
   static_assert(NW * 16 * (D + 2) * 4 <= kRingBytes, "merge area must fit in the ring");
@@ -80,6 +79,15 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Asynchronous 16-byte copy to shared memory, and the arrival on `bar` of this thread's
+// copies so far once they have landed (counted in the barrier's arrivals).
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Transposes an 8x8 matrix of 16-bit elements held two per lane.
@@ -121,29 +129,37 @@ __global__ void __launch_bounds__(NW * 32)
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
-    for (int i = 0; i < NW * NS; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < NW * NS; ++i) mbar_init(&bars[i], 33);  // the TMA bytes, and every lane's scales
     fence_barrier_init();
   }
   pdl_wait();
 
+  // Work units as in paged_decode_kernel. kList: a CTA's first unit is its own index, those
+  // past the grid are claimed from the counter one ahead (a launch with fewer units than
+  // CTAs leaves it alone: the atomics to one address took 1 us of 12). Looking the next
+  // unit up during this one's merge was 3% slower than at its start (more registers and
+  // waits in the merge), claiming two ahead 5% (uneven work at the end).
   __shared__ int claimed[2];
   int total = 0, next = 0;
   if constexpr (kList) {
-    const int cap = p.num_seqs * p.max_splits;
-    total = min(max(*p.item_count, 0), cap) * p.num_kv_heads;
-    if (threadIdx.x == 0) next = atomicAdd(p.item_next, 1);
+    // A unit list planned for another step (a caller error) can hold more entries than
+    // this launch's workspace holds, or sequences it does not have: the count is clamped
+    // to the capacity and every entry is checked.
+    total = min(max(*p.item_count, 0), p.num_seqs * p.max_splits) * p.num_kv_heads;
   }
   uint32_t gbase = 0;  // this warp's ring iterations so far
   for (int k = 0;; ++k) {
-    int split, b;
+    int split = 0, b;
     if constexpr (kList) {
-      if (threadIdx.x == 0) {
-        claimed[k & 1] = next;
-        next = atomicAdd(p.item_next, 1);
+      int u = blockIdx.x;
+      if (k > 0) {
+        if (threadIdx.x == 0) claimed[k & 1] = next;
+        __syncthreads();
+        u = claimed[k & 1];
       }
-      __syncthreads();
-      const int u = claimed[k & 1];
       if (u >= total) break;
+      const int grid = static_cast<int>(gridDim.x);
+      if (threadIdx.x == 0) next = total > grid ? grid + atomicAdd(p.item_next, 1) : total;
       h = u % p.num_kv_heads;
       const int item = p.items[u / p.num_kv_heads];
       if (item < 0 || item >= p.num_seqs * p.max_splits) {
@@ -154,17 +170,30 @@ __global__ void __launch_bounds__(NW * 32)
       b = item / p.max_splits;
     } else {
       if (k > 0) break;
-      split = 0;
       b = ordered_seq(p, blockIdx.z);
       if (b < 0) break;
     }
-
     // The first block ids need not wait for the length: entries below max_blocks exist, and
     // those past the context are dropped.
     const int first_blk = split * p.part_tokens / BS;
     const int32_t* bt = p.block_tables + static_cast<int64_t>(b) * p.bt_stride + first_blk;
     const int32_t early = first_blk + static_cast<int>(threadIdx.x) < p.max_blocks ? bt[threadIdx.x] : 0;
     int ctx = p.ctx_lens[b];
+    // The queries: loaded before the first stages' copies are issued where a CTA has one
+    // unit (14.3 against 14.9 us, Qwen geometry), after them in a list (1 us of 80).
+    uint2 qraw[kNT][kKSteps];
+    auto load_q = [&]() {
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        const bool real = nt * 8 + r < group;
+        const T* qrow = static_cast<const T*>(p.q) + b * p.q_stride +
+                        static_cast<int64_t>(h * group + (real ? nt * 8 + r : 0)) * D + 4 * q4;
+#pragma unroll
+        for (int kk = 0; kk < kKSteps; ++kk)
+          qraw[nt][kk] = real ? *reinterpret_cast<const uint2*>(qrow + 16 * kk) : make_uint2(0u, 0u);
+      }
+    };
+    if constexpr (!kList) load_q();
     if (ctx > p.max_blocks * BS) {
       if (threadIdx.x == 0 && split == 0) set_device_error(p.err, PS_DEVERR_LENGTH);
       ctx = 0;
@@ -177,7 +206,7 @@ __global__ void __launch_bounds__(NW * 32)
       }
       continue;
     }
-    if (split >= nsplit) continue;
+    if (split >= nsplit) continue;  // a stale list's entry
 
     const int t_begin = split * p.part_tokens;
     const int n_keys = min(ctx - t_begin, p.part_tokens);
@@ -193,34 +222,39 @@ __global__ void __launch_bounds__(NW * 32)
     }
     __syncthreads();
 
-    // Loads of warp-local iteration `it` (keys [32 j, 32 j + 32), j = warp + it NW):
-    // lane x of the first 4 kBoxes issues one copy (K codes, V codes, K scales,
-    // V scales of one box).
+    // Loads of warp-local iteration `it` (keys [32 j, 32 j + 32), j = warp + it NW): one
+    // lane issues the rows' TMA copies, sixteen copy four scales each (a bulk copy per box
+    // and scale pool would double the warp's issue time). A box past the partition's last
+    // block re-reads that block (its keys are masked).
     auto issue = [&](int it) {
       const int j = warp + it * NW;
       const int st = warp * NS + (gbase + it) % NS;
-      if (lane == 0) mbar_arrive_expect_tx(&bars[st], SM::kStageTx);
-      __syncwarp();
-      if (lane < 4 * kBoxes) {
-        const int x = lane >> 2;
-        const int what = lane & 3;
-        const int tok = j * kKeys + x * kBox;
-        // A box past the partition's last block re-reads that block (its keys are masked).
-        const int bi = min(tok / BS, nblk - 1);
-        const int64_t row = (static_cast<int64_t>(table[bi]) * p.num_kv_heads + h) * BS + tok % BS;
-        if (what < 2) {
-          tma_load_2d(smem + (st * 2 + what) * SM::kTileBytes + x * kBox * D, what ? &vmap : &kmap,
-                      &bars[st], 0, static_cast<int32_t>(row));
-        } else {
-          bulk_g2s(smem + SM::kScaleOffset + (st * 2 + what - 2) * kKeys * 4 + x * kBox * 4,
-                   (what == 2 ? qp.k_scale : qp.v_scale) + row, kBox * 4, &bars[st]);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars[st], 2 * SM::kTileBytes);
+#pragma unroll
+        for (int x = 0; x < kBoxes; ++x) {
+          const int tok = j * kKeys + x * kBox;
+          const int32_t row =
+              (table[min(tok / BS, nblk - 1)] * p.num_kv_heads + h) * BS + tok % BS;
+          uint8_t* dst = smem + st * 2 * SM::kTileBytes + x * kBox * D;
+          tma_load_2d(dst, &kmap, &bars[st], 0, row);
+          tma_load_2d(dst + SM::kTileBytes, &vmap, &bars[st], 0, row);
         }
       }
+      if (lane < 16) {
+        const int tok = j * kKeys + (lane & 7) * 4;
+        const int64_t row =
+            static_cast<int64_t>(table[min(tok / BS, nblk - 1)] * p.num_kv_heads + h) * BS + tok % BS;
+        cp_async16(smem + SM::kScaleOffset + st * 2 * kKeys * 4 + lane * 16,
+                   (lane < 8 ? qp.k_scale : qp.v_scale) + row);
+      }
+      cp_async_arrive(&bars[st]);
     };
 #pragma unroll
     for (int it = 0; it < NS; ++it)
       if (warp + it * NW < nchunk) issue(it);
 
+    if constexpr (kList) load_q();
     // Q as the B operand: lane holds head n = lane/4 of each head tile, dims
     // 16 kk + 4 q4 .. + 3 of k step kk, as fp16 times 2^-e_head. The factor that
     // turns an S element of heads 2 q4, 2 q4 + 1 into log2 units goes to qs.
@@ -228,16 +262,12 @@ __global__ void __launch_bounds__(NW * 32)
     float2 qs[kNT];
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      const bool real = nt * 8 + r < group;
-      const T* qrow = static_cast<const T*>(p.q) + b * p.q_stride +
-                      static_cast<int64_t>(h * group + (real ? nt * 8 + r : 0)) * D + 4 * q4;
       float2 x[kKSteps][2];
       float mx = 0.f;
 #pragma unroll
       for (int kk = 0; kk < kKSteps; ++kk) {
-        const uint2 v = real ? *reinterpret_cast<const uint2*>(qrow + 16 * kk) : make_uint2(0u, 0u);
-        x[kk][0] = unpack2<T>(v.x);
-        x[kk][1] = unpack2<T>(v.y);
+        x[kk][0] = unpack2<T>(qraw[nt][kk].x);
+        x[kk][1] = unpack2<T>(qraw[nt][kk].y);
         mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[kk][0].x), fabsf(x[kk][0].y)),
                              fmaxf(fabsf(x[kk][1].x), fabsf(x[kk][1].y))));
       }
