@@ -432,10 +432,6 @@ __global__ void __launch_bounds__(NW * 32)
     float mmax = -INFINITY;
 #pragma unroll
     for (int w = 0; w < NW; ++w) mmax = fmaxf(mmax, ms[w * R + g]);
-    const SharedRows shared(p, b, h, g);
-    if constexpr (kShared) {
-      for (int s = 0; s < npre; ++s) mmax = fmaxf(mmax, shared.ml(p, s).x);
-    }
     float lsum = 0.f;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -449,19 +445,7 @@ __global__ void __launch_bounds__(NW * 32)
       acc[2] += ov.z * sc;
       acc[3] += ov.w * sc;
     }
-    if constexpr (kShared) {
-#pragma unroll 8
-      for (int s = 0; s < npre; ++s) {
-        const float2 ml = shared.ml(p, s);
-        const float4 ov = shared.o<D>(p, s, d / 4);
-        const float sc = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mmax);
-        lsum += ml.y * sc;
-        acc[0] += ov.x * sc;
-        acc[1] += ov.y * sc;
-        acc[2] += ov.z * sc;
-        acc[3] += ov.w * sc;
-      }
-    }
+    if constexpr (kShared) merge_shared<D>(p, SharedRows(p, b, h, g), npre, d / 4, mmax, lsum, acc);
     const float inv = (lsum > 0.f) ? 1.f / lsum : 0.f;
     const int qh = h * group + g;
     if (single) {
