@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -163,3 +164,21 @@ def test_shared_workspace_and_pieces():
     for sizes, hq, hkv, keys in (([8], 64, 8, 32768), ([17, 3, 40], 14, 2, 2000), ([1], 8, 8, 64), ([500], 16, 1, 100000)):
         split = ops.shared_split_keys(sizes, hq, hkv, keys, 148)
         assert split % 128 == 0 and 0 <= split < keys
+
+
+@pytest.mark.parametrize("qmax", [448.0, 127.0])
+def test_division_by_the_code_range(qmax):
+    """fma(x, hi, x * lo) with hi + lo ~ 1 / qmax is x / qmax, rounded once, for every significand.
+
+    Both sides scale with powers of two, so x runs over the 2^23 integers of 24 bits. The sum
+    x * hi + fl(x * lo) is held exactly, as an integer multiple of 2^-36: hi is a multiple of 2^-32
+    (1/512 < hi), and a product rounded to 24 bits of at least 2^-13 one of 2^-36.
+    """
+    x = np.arange(1 << 23, 1 << 24, dtype=np.int64)
+    hi = np.float32(1.0 / qmax)
+    lo = np.float32(1.0 / qmax - float(hi))
+    small = (x.astype(np.float32) * lo).astype(np.float64) * 2.0**36
+    assert np.array_equal(small, np.rint(small))
+    exact = x * np.int64(float(hi) * 2.0**36) + small.astype(np.int64)
+    fma = exact.astype(np.float32) * np.float32(2.0**-36)  # one rounding; the scaling is exact
+    assert np.array_equal(fma, x.astype(np.float32) / np.float32(qmax))
