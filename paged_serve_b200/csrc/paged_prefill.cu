@@ -37,10 +37,10 @@
 // kShared: the shared-prefix pass of a decode step (shared_prefix.h). The query rows
 // are the batch rows of a group, every key tile is a full one (no causal mask) and
 // every unit leaves partials. 256 rows of 4 heads over 8192 keys, 8 KV heads, D 128 (34
-// GFLOP): 43 us of this kernel under ncu's cold caches in four pieces, 0.47 of the
-// burst peak, bound by the per-tile chain and, with 16 key tiles a unit, by a unit's
+// GFLOP): 51 us of this kernel under ncu (cold caches, 1.4 GHz) in four pieces, 0.40 of
+// the burst peak, bound by the per-tile chain and, with 16 key tiles a unit, by a unit's
 // start and end (about five key tiles' time). 8 rows of 8 heads over 32768 keys (134 MB):
-// 36 us in 16 pieces of paired tiles, 0.57 of the copy peak.
+// 42 us in 16 pieces of paired tiles, 0.50 of the copy peak.
 //
 // All waits are bounded; a timeout sets PS_DEVERR_TIMEOUT and a shared abort
 // flag so every role leaves its loop, drains its in-flight copies / MMAs and
