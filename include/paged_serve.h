@@ -489,8 +489,8 @@ PS_API int64_t ps_paged_prefill_workspace_bytes(int num_seqs, int max_q_len, int
  * split_tokens cuts the keys behind the prefixes; seq_order orders sequences by them.
  * workspace: ps_paged_decode_shared_workspace_bytes(...) bytes, 256-byte aligned, one
  *   call at a time.
- * Errors: a shared length that breaks these rules sets PS_DEVERR_LENGTH (the outputs
- * of the rows concerned are then unspecified). Keys at or past ctx_lens[b] are not
+ * Errors: a shared length or a group that breaks these rules sets PS_DEVERR_LENGTH (the
+ * outputs of the rows concerned are then unspecified). Keys at or past ctx_lens[b] are not
  * used, whatever their rows hold.
  */
 PS_API int ps_paged_decode_shared(void* out, int64_t out_seq_stride, const void* query,

@@ -104,6 +104,7 @@ constexpr int kThreads = 384;
 constexpr int kWarpTma = 8;
 constexpr int kWarpMma = 9;
 constexpr int kWarpTmaV = 10;  // paired shared-prefix tiles only
+constexpr int kWarpCheck = 11;  // shared-prefix pass only
 constexpr uint32_t kRegsSoftmax = 192;
 constexpr uint32_t kRegsOther = 64;
 constexpr int kRegPoolNeeded = 256 * kRegsSoftmax + 128 * kRegsOther;
@@ -502,6 +503,35 @@ __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* b
 }
 
 // BS = tokens per KV block (8, 16 or 32): a 128-key tile is 128/BS block boxes.
+// Shared-prefix pass: sets an error bit unless the groups are in order and every row with
+// a prefix is in one whose rows all have its length (a row outside would merge partials that
+// nothing has written). As the groups leave no gaps, that is: a row whose length
+// differs from the row's before it starts a group, or ends the last one with nothing shared.
+// Rows go to the lanes of one otherwise idle warp per CTA.
+__device__ __forceinline__ void check_groups(const PrefillParams& p, int lane) {
+  const int step = static_cast<int>(gridDim.x) * 32;
+  const int first = static_cast<int>(blockIdx.x) * 32 + lane;
+  bool bad = false;
+  for (int g = first; g < p.num_seqs; g += step) bad |= p.q_starts[g] > p.q_starts[g + 1];
+  const int end = p.q_starts[p.num_seqs];
+  for (int i = first; i < p.num_rows; i += step) {
+    const int pre = p.ctx_lens[i];
+    const int before = i > 0 ? p.ctx_lens[i - 1] : 0;
+    if (i >= end) {
+      bad |= pre != 0;
+    } else if (pre != before) {
+      int lo = 0, hi = p.num_seqs;  // the first group that starts at i or behind
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (p.q_starts[mid] < i) lo = mid + 1;
+        else hi = mid;
+      }
+      bad |= p.q_starts[lo] != i;
+    }
+  }
+  if (bad) set_device_error(p.err, PS_DEVERR_LENGTH);
+}
+
 template <typename T, int D, int BS, bool kSplit, bool kShared>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap qmap,
@@ -872,7 +902,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (leader) umma_commit(&bars[C::kBarDone]);
     __syncwarp();
     (void)drain_wait(&bars[C::kBarDone], 0);
-  }  // warps 10 (unless paired) and 11 have no role
+  } else if (kShared && warp == kWarpCheck) {
+    check_groups(p, lane);
+  }  // warps 10 (unless paired) and 11 (unless shared) have no role
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ------------------------------------------------------------ softmax + epilogue

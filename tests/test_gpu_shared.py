@@ -170,6 +170,34 @@ def test_bad_lengths_are_reported():
     assert code(tables=bad) & _lib.PS_DEVERR_BLOCK_ID
 
 
+def test_rows_outside_their_group_are_reported():
+    pre, starts, lens, tables, nb = _case([(2, 64), (2, 128), (3, 0), (1, 32)], [10, 20, 30, 40, 5, 6, 7, 8], 16)
+    pools = random_pool(nb, 2, 16, 64, torch.bfloat16, DEV, seed=6)
+    q = torch.randn((8, 8, 64), device=DEV).to(torch.bfloat16)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+
+    def code(pre=pre, starts=starts, max_group=3):
+        err.zero_()
+        for group in (max_group, 8):
+            for split in (0, 32):
+                ops.paged_decode_shared(q, *pools, tables.to(DEV), _i32(lens), _i32(starts), _i32(pre), group,
+                                        128, 0.125, split_keys=128, split_tokens=split, device_error=err)
+        return int(err)
+
+    length = _lib.PS_DEVERR_LENGTH
+    assert code() == 0
+    assert code(starts=[0, 2, 4, 4, 4, 7, 8]) == 0  # groups without rows
+    assert code(starts=[0, 2, 3, 4, 7, 8]) == 0  # neighbours of one length in two groups
+    assert code(pre=[0, 0, 128, 128, 0, 0, 0, 0], starts=[2, 4]) == 0  # rows in no group
+    assert code(pre=[0] * 8, starts=[3, 3]) == 0
+    assert code(starts=[0, 2, 4, 7]) == length  # the last row's prefix in no group
+    assert code(starts=[2, 4, 7, 8]) == length  # the first rows'
+    assert code(pre=[0, 64, 128, 128, 0, 0, 0, 32]) == length  # the first row of a group has none
+    assert code(pre=[64, 64, 128, 128, 0, 16, 0, 32]) == length
+    assert code(starts=[0, 2, 4, 3, 7, 8]) == length  # not in order
+    assert code(pre=[64] * 8, starts=[0, 7], max_group=7) == length
+
+
 def test_streams_and_graphs():
     """Another stream, and two captured calls that share a workspace replayed in turn,
     with the inputs of the calls written by the kernels just before them."""
