@@ -223,7 +223,8 @@ PS_API int64_t ps_paged_decode_workspace_bytes(int num_seqs, int num_q_heads, in
  *   ctx_lens, and the counter the persistent decode CTAs claim units from. Every call
  *   rewrites all of it before reading it (no clearing needed); calls that share one
  *   workspace must not overlap on the GPU.
- * Softmax and accumulation are fp32; the output is rounded once to dtype.
+ * Softmax and accumulation are fp32; the output is rounded once to dtype. Keys at or past
+ * ctx_lens[b] are not used, whatever their rows hold (NaN among it).
  */
 PS_API int ps_paged_decode(void* out, int64_t out_seq_stride, const void* query,
                     int64_t query_seq_stride, const void* k_pool, const void* v_pool,

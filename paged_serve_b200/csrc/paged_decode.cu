@@ -306,6 +306,13 @@ __global__ void __launch_bounds__(NW * 32)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (tok0 + tk[e] >= t_end) x[e] = y[e] = -INFINITY;
+      // Values behind the last key become 0 in shared memory: what their rows hold (NaN
+      // among it) must not meet a probability of 0.
+      const int left = t_end - tok0;
+      for (int i = lane; i < (kChunk - left) * (D / 8); i += 32)
+        *reinterpret_cast<uint4*>(ring + st * SM::kStageBytes + G::kTileBytes +
+                                  G::off(left + i / (D / 8), i % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
+      __syncwarp();
     }
     float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -345,25 +352,10 @@ __global__ void __launch_bounds__(NW * 32)
     }
 
     // ---- O += P V
-    // kShared: values of keys past the end become 0, whatever their rows hold (this
-    // lane's keys are 2 q4, 2 q4 + 1 in the low and high half of b00/b10, and the
-    // same plus 8 in b01/b11).
-    uint32_t live0 = 0xffffffffu, live1 = 0xffffffffu;
-    if constexpr (kShared) {
-      const int k0 = t_end - tok0 - 2 * q4;
-      live0 = k0 >= 2 ? 0xffffffffu : k0 == 1 ? 0x0000ffffu : 0u;
-      live1 = k0 >= 10 ? 0xffffffffu : k0 == 9 ? 0x0000ffffu : 0u;
-    }
 #pragma unroll
     for (int jj = 0; jj < kNTiles / 2; ++jj) {
       uint32_t b00, b01, b10, b11;
       ldsm_x4_t(vbase + G::off(pv_t, 2 * jj + pv_c), b00, b01, b10, b11);
-      if constexpr (kShared) {
-        b00 &= live0;
-        b01 &= live1;
-        b10 &= live0;
-        b11 &= live1;
-      }
       Mma<T>::run(o[2 * jj], pa0, pa1, pa2, pa3, b00, b01);
       Mma<T>::run(o[2 * jj + 1], pa0, pa1, pa2, pa3, b10, b11);
     }

@@ -135,6 +135,19 @@ def test_nothing_shared_is_paged_decode():
     _check(out, q, pools, tables, lens, "nothing shared", HALF[torch.float16])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,d,bs", [(32, 8, 128, 16), (14, 2, 64, 8), (16, 1, 64, 32)])
+@pytest.mark.parametrize("split", [0, 32])
+def test_nothing_shared_ignores_stale_rows(dtype, hq, hkv, d, bs, split):
+    lens = [1, 7, 8, 0, 15, 16, 17, 33, 130, 255]
+    pre, starts, lens, tables, nb = _case([(len(lens), 0)], lens, bs, seed=9)
+    pools = random_pool(nb, hkv, bs, d, dtype, DEV, seed=10)
+    _spoil_tails(pools, tables, lens)
+    q = torch.randn((len(lens), hq, d), device=DEV).to(dtype)
+    out = _shared(q, pools, tables, lens, pre, starts, split=split)
+    _check(out, q, pools, tables, lens, "nothing shared", HALF[dtype])
+
+
 def test_bad_lengths_are_reported():
     pre, starts, lens, tables, nb = _case([(2, 64), (2, 128)], [10, 20, 30, 40], 16)
     pools = random_pool(nb, 2, 16, 64, torch.bfloat16, DEV, seed=6)
