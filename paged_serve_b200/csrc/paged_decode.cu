@@ -307,7 +307,8 @@ __global__ void __launch_bounds__(NW * 32)
       for (int e = 0; e < 4; ++e)
         if (tok0 + tk[e] >= t_end) x[e] = y[e] = -INFINITY;
       // Values behind the last key become 0 in shared memory: what their rows hold (NaN
-      // among it) must not meet a probability of 0.
+      // among it) must not meet a probability of 0. (Masking the fragments of every chunk
+      // instead: 17.9 against 16.9 us, small groups under short prefixes.)
       const int left = t_end - tok0;
       for (int i = lane; i < (kChunk - left) * (D / 8); i += 32)
         *reinterpret_cast<uint4*>(ring + st * SM::kStageBytes + G::kTileBytes +
