@@ -477,8 +477,8 @@ PS_API int64_t ps_paged_prefill_workspace_bytes(int num_seqs, int max_q_len, int
  *
  * Arguments as ps_paged_decode_ordered, and:
  * group_starts: [num_groups + 1] int32, group g = batch rows
- *   [group_starts[g], group_starts[g + 1]); at most max_group rows each (groups that
-   share nothing may be longer).
+ *   [group_starts[g], group_starts[g + 1]); at most max_group rows each (groups
+ *   that share nothing may be longer).
  * shared_lens: [num_seqs] int32, the shared keys of each row: a multiple of
  *   block_size, at most ctx_lens[b] and max_shared, the same for all rows of a
  *   group, 0 for a row that shares nothing (such rows need no group; every row with
@@ -524,9 +524,10 @@ PS_API int64_t ps_paged_decode_shared_workspace_bytes(int num_seqs, int num_q_he
  *     scale = max(max|x| / qmax, 2^-126),  qmax = 448 (PS_CODE_E4M3) or 127 (PS_CODE_INT8)
  *     code  = round(x * (1 / scale)), ties to even
  * every operation rounded to float32, so the codes are reproducible to the bit.
- * A row with a NaN or an infinity gets a NaN scale: all its values read back as NaN. Blocks move with ps_copy_blocks / ps_swap_blocks: codes with
- * block_bytes = num_kv_heads*block_size*head_dim, scales (called the same way with the
- * scale pools) with num_kv_heads*block_size*4.
+ * A row with a NaN or an infinity gets a NaN scale: all its values read back as NaN.
+ * Blocks move with ps_copy_blocks / ps_swap_blocks: codes with block_bytes =
+ * num_kv_heads*block_size*head_dim, scales (called the same way with the scale pools)
+ * with num_kv_heads*block_size*4.
  */
 
 /*
