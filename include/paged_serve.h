@@ -593,9 +593,12 @@ PS_API int ps_cache_read_quant(const void* k_pool, const void* v_pool, const flo
  * ps_paged_decode_listed (may be NULL with num_listed < 0); num_listed < 0 = all
  * num_seqs sequences, else the entries of seq_list to run; planned != 0 = the unit
  * list for these lengths, order and geometry is already in the workspace
- * (ps_paged_decode_plan); it covers all sequences, so num_listed must be negative. Keys at or past ctx_lens[b] are not
- * used, whatever their rows and scales hold. Scores, softmax and accumulation are
- * float32; probabilities times V scales are rounded to fp16 for the second product.
+ * (ps_paged_decode_plan); it covers all sequences, so num_listed must be negative. Keys
+ * at or past ctx_lens[b] are not used, whatever their rows and scales hold. Scores,
+ * softmax and accumulation are float32; probabilities times V scales are rounded to fp16
+ * for the second product (a probability below 2^-126 of the largest counts as 0). As in
+ * ps_paged_decode the sum of p |v| before the division, p = 1 at the largest score, must stay
+ * in float32's range.
  */
 PS_API int ps_paged_decode_quant(void* out, int64_t out_seq_stride, const void* query,
                                  int64_t query_seq_stride, const void* k_pool, const void* v_pool,

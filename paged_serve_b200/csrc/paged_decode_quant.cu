@@ -16,7 +16,12 @@
 //   P'_n = 2^(s_n + log2 b_n - M + 7)
 // Both maxima move only when passed by 8 (2^8), so P' is below 2^15.2 and a term
 // keeps fp16's full precision down to 2^-21 of the largest one; O is rescaled, in
-// fp32, when M moves.
+// fp32, when M moves. P' is formed as (p_n F) (b_n H) with p_n = 2^(s_n - m) and
+// F H = f = 2^(m - M + 7), F = max(f, 1): p_n is at most 2^8 and b_n below 2^121, so no
+// factor overflows as long as f is at most 2^119. That is M >= m - 112, which M is held to:
+// only where every value is below 2^-112 of what a probability of 1 weighs do terms start lower
+// than 2^7. (b_n f in one product was infinite where the top key's values were zeros and
+// others', far below it, were not, and a NaN where their p_n was 0.) A p_n below 2^-126 is 0.
 //
 // Work decomposition as in paged_decode.cu: one CTA per (KV head, sequence), or
 // persistent CTAs claiming (KV head, partition) units; each warp owns a ring of
@@ -374,12 +379,12 @@ __global__ void __launch_bounds__(NW * 32)
               u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, o_));
             }
             const float m_new = fmaxf(m_, t);
-            const float mv_new = fmaxf(mv_, u);
+            const float mv_new = fmaxf(fmaxf(mv_, u), m_new - 112.f);
             l_ *= m_new == -INFINITY ? 1.f : ex2(m_ - m_new);
             const float alpha = mv_new == -INFINITY ? 1.f : ex2(mv_ - mv_new);
             m_ = m_new;
             mv_ = mv_new;
-            f_ = ex2(fminf(m_new - mv_new + 7.f, 120.f));
+            f_ = ex2(m_new - mv_new + 7.f);
             return alpha;
           };
           const float al0 = raise(top[nt].x, topv[nt].x, m[nt].x, mv[nt].x, l[nt].x, f[nt].x);
@@ -401,6 +406,12 @@ __global__ void __launch_bounds__(NW * 32)
       constexpr bool kTwoTerms = std::is_same<T, __half>::value;
       uint32_t pb[2][kNT][2];
       [[maybe_unused]] uint32_t pl[2][kNT][2];
+      float2 up[kNT], down[kNT];  // F and H
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        up[nt] = make_float2(fmaxf(f[nt].x, 1.f), fmaxf(f[nt].y, 1.f));
+        down[nt] = make_float2(fminf(f[nt].x, 1.f), fminf(f[nt].y, 1.f));
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -408,7 +419,8 @@ __global__ void __launch_bounds__(NW * 32)
           const float2 z = __fadd2_rn(x[i][nt], make_float2(-m[nt].x, -m[nt].y));
           const float2 pr = make_float2(ex2(z.x), ex2(z.y));
           l[nt] = __fadd2_rn(l[nt], pr);
-          const float2 pv = __fmul2_rn(pr, __fmul2_rn(make_float2(vs[i], vs[i]), f[nt]));
+          const float2 pv = __fmul2_rn(__fmul2_rn(pr, up[nt]),
+                                       __fmul2_rn(make_float2(vs[i], vs[i]), down[nt]));
           const uint32_t hi = pack2<__half>(pv);
           pb[i >> 1][nt][i & 1] = transpose8x8(hi);
           if constexpr (kTwoTerms) {

@@ -379,6 +379,52 @@ def test_on_another_stream_and_in_graphs():
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want2)
 
 
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,at", [(64, 0), (128, 45), (64, 99)])
+def test_decode_of_a_top_key_with_a_row_of_zeros(code, dtype, d, at):
+    """The key with nearly all of the softmax has zeros for values (their scale 2^-126), and
+    the others, 2^gap below it, have values of any size: finite, and the attention of the rest.
+
+    Beside the roundings of assert_within, in units of the largest probability: a probability
+    below 2^-126 may count as 0 (n 2^-126 max|v| in all); P b is held to 2^-25 2^-119 or better, which
+    meets codes of at most 448 (n 2^-135); the output's smallest step."""
+    hq, bs, n = 8, 16, 100
+    nb = (n + bs - 1) // bs
+    g = _gen(30)
+    tables = torch.arange(nb, dtype=torch.int32).view(1, nb)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    q = torch.randn((1, hq, d), device=DEV, generator=g) * 0.1
+    q[..., 0] = 1.0
+    q = q.to(dtype)
+    k = torch.randn((nb, 1, bs, d), device=DEV, generator=g)
+    k[..., 0] = 0.0
+    v = torch.randn((nb, 1, bs, d), device=DEV, generator=g)
+    v /= v.abs().amax(-1, keepdim=True)
+    v[at // bs, 0, at % bs] = 0.0
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # the output's smallest step
+    for gap in (0, 40, 100, 112, 118, 125, 127, 140, 210, 250):
+        k[at // bs, 0, at % bs] = 0.0
+        k[at // bs, 0, at % bs, 0] = gap * math.log(2.0)
+        kp, ks = quantise(k, code)
+        for size in (1e-30, 1.0, 6e4, 1e20, 1e30, 1e38):
+            vp, vs = quantise(v * size, code)
+            out = ops.paged_decode_quant(q, kp, vp, ks, vs, tables.to(DEV), lens, 1.0)
+            kk = dequantise(sequence(kp, tables[0].to(DEV), n), sequence(ks, tables[0].to(DEV), n))
+            vv = dequantise(sequence(vp, tables[0].to(DEV), n), sequence(vs, tables[0].to(DEV), n))
+            ref, weight = attend(q[0], kk, vv, 1.0)
+            # refused by the documentation: sum(p |v|) in units of the top probability, up to
+            # 100 x 1e38 here, is formed in float32 (3.4e38); or beyond the output's range
+            p_v = torch.softmax(torch.einsum("hd,nd->hn", q[0].double(), kk[0]), -1)
+            if float((p_v / p_v.amax(-1, keepdim=True) @ vv[0].abs()).max()) > 2.0**127 or                     float(ref.abs().max()) > torch.finfo(dtype).max / 2:
+                continue
+            bound = (torch.finfo(dtype).eps / 2 * ref.abs() + 1.1 * 2.0**-11 * weight
+                     + 2.0**-21 * weight.amax(-1, keepdim=True) + tiny / 2
+                     + n * (2.0**-126 * float(vv.abs().max()) + 2.0**-135))
+            err = (out[0].double() - ref).abs()
+            assert (err <= bound).all(), (gap, size, float((err / bound).nan_to_num(nan=math.inf).max()))
+
+
 # ------------------------------------------------------------------ together
 @pytest.mark.parametrize("code", CODES)
 def test_prompt_then_decode_steps(code):
