@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(NW * 32)
   const bool any_keys = ctx > 0;
   int pre = 0;
   if constexpr (kShared) {
-    if (any_keys) pre = shared_prefix(p, b, ctx, threadIdx.x == 0);
+    // Also without keys: a prefix is longer than such a sequence.
+    pre = shared_prefix(p, b, max(ctx, 0), threadIdx.x == 0);
     ctx -= pre;  // from here on: the sequence's own keys, behind the prefix
   }
   const int nsplit = (ctx + p.part_tokens - 1) / p.part_tokens;

@@ -211,6 +211,27 @@ def test_rows_outside_their_group_are_reported():
     assert code(pre=[64] * 8, starts=[0, 7], max_group=7) == length
 
 
+@pytest.mark.parametrize("split", [0, 32])
+def test_a_prefix_of_a_sequence_without_keys_is_reported(split):
+    """A row of a group with a prefix but no keys at all breaks the rule as one with too few does."""
+    pre, starts, lens, tables, nb = _case([(2, 64), (2, 0)], [10, 20, 30, 0], 16)
+    pools = random_pool(nb, 2, 16, 64, torch.bfloat16, DEV, seed=11)
+    q = torch.randn((4, 8, 64), device=DEV).to(torch.bfloat16)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = _shared(q, pools, tables, lens, pre, starts, 128, split, device_error=err)
+    assert int(err) == 0 and (out[3] == 0).all()
+    for empty in (0, -5):
+        for row in (0, 1):
+            err.zero_()
+            bad = list(lens)
+            bad[row] = empty
+            _shared(q, pools, tables, bad, pre, starts, 128, split, device_error=err)
+            assert int(err) == _lib.PS_DEVERR_LENGTH, (empty, row)
+        err.zero_()  # without a prefix a row without keys is no error
+        out = _shared(q, pools, tables, [*lens[:3], empty], pre, starts, 128, split, device_error=err)
+        assert int(err) == 0 and (out[3] == 0).all()
+
+
 def test_streams_and_graphs():
     """Another stream, and two captured calls that share a workspace replayed in turn,
     with the inputs of the calls written by the kernels just before them."""
