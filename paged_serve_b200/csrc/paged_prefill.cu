@@ -147,6 +147,7 @@ struct PrefillParams {
   // most) tiles A and B hold the same rows and take even and odd key tiles, so the
   // softmax of one still runs beside the other's MMAs, and a piece leaves two partials.
   bool paired;
+  int max_group;
   float scale_log2;
   int32_t* err;
 };
@@ -203,7 +204,7 @@ __device__ __forceinline__ bool decode_item(const PrefillParams& p, int u, Item&
     if (w.ctx == 0) return false;  // nothing shared
     const int64_t room = static_cast<int64_t>(p.splits) * p.split_tiles * kN;  // pieces' keys
     if (w.ctx < 0 || w.ctx > p.max_blocks * p.block_size || w.ctx > room ||
-        w.ctx % p.block_size != 0 || w.q_len > nq * (p.paired ? 1 : 2) * p.tokens_per_tile) {
+        w.ctx % p.block_size != 0 || w.q_len > p.max_group) {  // the tiles hold max_group rows
       if (report) set_device_error(p.err, PS_DEVERR_LENGTH);
       return false;
     }
@@ -1231,6 +1232,7 @@ int launch_shared_prefix(const SharedPrefix& a, cudaStream_t s) {
   p.block_size = a.block_size;
   p.num_seqs = a.num_groups;
   p.paired = a.paired;
+  p.max_group = a.max_group;
   p.num_q_tiles = a.paired ? 1 : (a.max_group + 2 * tpt - 1) / (2 * tpt);
   const int64_t items = static_cast<int64_t>(p.num_q_tiles) * a.num_kv_heads * a.num_groups;
   if (items * a.pieces >= (int64_t(1) << 31))

@@ -232,6 +232,22 @@ def test_a_prefix_of_a_sequence_without_keys_is_reported(split):
         assert int(err) == 0 and (out[3] == 0).all()
 
 
+@pytest.mark.parametrize("hq,hkv", [(4, 4), (8, 2), (32, 2)])
+def test_a_group_longer_than_max_group_is_reported(hq, hkv):
+    """Also where a query tile would hold the rows; a long group that shares nothing is none."""
+    pre, starts, lens, tables, nb = _case([(3, 64), (5, 0), (2, 32)], [9] * 10, 16)
+    pools = random_pool(nb, hkv, 16, 64, torch.bfloat16, DEV, seed=12)
+    q = torch.randn((10, hq, 64), device=DEV).to(torch.bfloat16)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for max_group, want in ((1, _lib.PS_DEVERR_LENGTH), (2, _lib.PS_DEVERR_LENGTH), (3, 0), (10, 0)):
+        err.zero_()
+        out = ops.paged_decode_shared(q, *pools, tables.to(DEV), _i32(lens), _i32(starts), _i32(pre), max_group, 64,
+                                      0.125, device_error=err)
+        assert int(err) == want, max_group
+        if not want:
+            _check(out, q, pools, tables, lens, f"max_group {max_group}")
+
+
 def test_streams_and_graphs():
     """Another stream, and two captured calls that share a workspace replayed in turn,
     with the inputs of the calls written by the kernels just before them."""
