@@ -853,10 +853,9 @@ class PagedCudaBackend(AttentionBackend):
                 device_error=err, seq_order=md.seq_order, planned=md.decode_planned,
             ).view(b, 1, hq, d)
         flat = query.reshape(b * tq, hq, d)
-        out = torch.empty_like(flat)
-        q_lens = md.q_lens
+        q_lens, out = md.q_lens, None  # the prefill makes its own output: zeros in padding rows
         if md.decode_list is not None:
-            q_lens = md.prefill_q_lens
+            q_lens, out = md.prefill_q_lens, torch.empty_like(flat)
             ops.paged_decode_quant(
                 flat.view(b, tq, hq, d)[:, tq - 1], *cache, md.block_tables, md.ctx_lens,
                 self.scale, self.split_tokens, out=out.view(b, tq, hq, d)[:, tq - 1],
@@ -867,10 +866,10 @@ class PagedCudaBackend(AttentionBackend):
             ops.cache_read_quant(*cache, md.block_tables[:, :w], md.read_lens, k, v,
                                  md.read_tables, err)
             split = md.prefill_split_keys
-            ops.paged_prefill(flat, k, v, md.read_tables, md.q_starts, q_lens, md.ctx_before, tq,
-                              self.scale, out=out, device_error=err, split_keys=split,
-                              workspace=self._prefill_ws if split else None,
-                              max_keys=md.key_len)
+            out = ops.paged_prefill(flat, k, v, md.read_tables, md.q_starts, q_lens,
+                                    md.ctx_before, tq, self.scale, out=out, device_error=err,
+                                    split_keys=split, workspace=self._prefill_ws if split else None,
+                                    max_keys=md.key_len)
         return out.view(b, tq, hq, d)
 
     def write_kv_rope(

@@ -237,6 +237,27 @@ def test_static_engine_over_an_8_bit_cache(code, use_tables):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("code", [None, *CODES])
+def test_a_prefill_leaves_zeros_in_padding_rows(code):
+    """Left-padded prompts: the rows before a prompt are zeros, whatever the memory held before."""
+    prompts = [37, 5, 64]
+    b, tq, hq, hkv, d = 3, 64, 8, 2, 128
+    be = PagedCudaBackend(MODEL, device=DEV, dtype=torch.bfloat16, kv_codes=code)
+    be.allocate(b, 128)
+    mask = torch.zeros((b, tq), dtype=torch.bool, device=DEV)
+    for i, n in enumerate(prompts):
+        mask[i, tq - n:] = True
+    md = be.begin_step(StepInput(query_len=tq, context_len=0, seq_lens=mask.sum(1).to(torch.int32),
+                                 padding_mask=mask, is_prefill=True))
+    q, k, v = (torch.randn((b, tq, h, d), device=DEV).to(torch.bfloat16) for h in (hq, hkv, hkv))
+    for _ in range(2):
+        junk = [torch.full((b * tq, hq, d), float("nan"), device=DEV, dtype=torch.bfloat16) for _ in range(4)]
+        del junk
+        out = be.forward(0, q, k, v, md)
+        assert (out[~mask] == 0).all() and out[mask].isfinite().all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("code", CODES)
 def test_decode_graph_over_an_8_bit_cache(code):
     """DecodeGraph replays equal eager steps, with growing contexts and an inactive row."""
