@@ -92,13 +92,17 @@ class PagedMetadata(AttentionMetadata):
     # begin_step / begin_plan / the static loaders); forward then skips the plan.
     decode_planned: bool = False
     # Prefill steps with few query tiles over long contexts: keys per split-K
-    # piece (ops.prefill_split_keys; 0 = items run whole).
+    # piece (ops.prefill_split_keys; 0 = items run whole), and their workspace. A step keeps
+    # the buffers it was planned with (here, read_pools, shared_ws): the backend's own grow
+    # with later steps, while a graph captured with this one holds these addresses.
     prefill_split_keys: int = 0
+    prefill_ws: torch.Tensor | None = None
     # 8-bit cache, steps that prefill: where each prefilling sequence's tokens are read
     # back to (int32 [B, W] blocks of the 16-bit scratch pool) and how many (int32 [B],
     # 0 for the others).
     read_tables: torch.Tensor | None = None
     read_lens: torch.Tensor | None = None
+    read_pools: tuple[torch.Tensor, torch.Tensor] | None = None  # the 16-bit scratch (K, V)
     # Decode steps whose neighbours share leading blocks: int32 [groups + 1] first rows,
     # int32 [B] shared tokens, the largest of each, and the keys per piece.
     group_starts: torch.Tensor | None = None
@@ -107,6 +111,7 @@ class PagedMetadata(AttentionMetadata):
     max_shared: int = 0
     shared_split_keys: int = 0
     shared_split_tokens: int = 0  # split-K of the keys behind the prefixes, where any needs it
+    shared_ws: torch.Tensor | None = None
 
 
 class PagedCudaBackend(AttentionBackend):
@@ -347,7 +352,7 @@ class PagedCudaBackend(AttentionBackend):
         elif tq > 1:
             keys = self._plan_prefill_split(self._prefill_items(None, b, tq), tq, b, key_len)
             if keys:
-                md = dataclasses.replace(md, prefill_split_keys=keys)
+                md = dataclasses.replace(md, prefill_split_keys=keys, prefill_ws=self._prefill_ws)
         if self.kv_codes is not None and tq > 1:
             w = -(-key_len // bs)
             rows = torch.arange(b * w, dtype=torch.int32, device=dev).view(b, w)
@@ -370,7 +375,8 @@ class PagedCudaBackend(AttentionBackend):
         src = md.block_tables
         if src.shape[1] < w:
             tables = tables[:, : src.shape[1]].contiguous()
-        return dataclasses.replace(md, read_tables=tables, read_lens=lens.contiguous())
+        return dataclasses.replace(md, read_tables=tables, read_lens=lens.contiguous(),
+                                   read_pools=self._scratch)
 
     def _decode_order(self, ctx_lens: torch.Tensor, query_len: int) -> torch.Tensor | None:
         """Longest-first order for the step's decode launches (one launch per step)."""
@@ -547,7 +553,7 @@ class PagedCudaBackend(AttentionBackend):
             keys = self._plan_prefill_split(self._prefill_items(plan.q_lens, b, tq), tq, b,
                                             max(lens))
             if keys:
-                md = dataclasses.replace(md, prefill_split_keys=keys)
+                md = dataclasses.replace(md, prefill_split_keys=keys, prefill_ws=self._prefill_ws)
         if read_w:
             md = self._plan_read(md, packed[extra : extra + b * read_w].view(b, read_w),
                                  packed[extra + b * read_w :], read_blocks)
@@ -587,7 +593,7 @@ class PagedCudaBackend(AttentionBackend):
         return dataclasses.replace(
             md, group_starts=starts, shared_lens=shared, max_group=max(sizes),
             max_shared=max_shared, shared_split_keys=keys, shared_split_tokens=split,
-            seq_order=ops.decode_order(md.ctx_lens - shared))
+            shared_ws=self._shared_ws, seq_order=ops.decode_order(md.ctx_lens - shared))
 
     # ------------------------------------------------------------------ CUDA graphs
     def static_decode_metadata(self, batch: int, width: int | None = None) -> PagedMetadata:
@@ -760,7 +766,7 @@ class PagedCudaBackend(AttentionBackend):
                 query.reshape(b, hq, d), k_pool, v_pool, md.block_tables, md.ctx_lens,
                 md.group_starts, md.shared_lens, md.max_group, md.max_shared, self.scale,
                 split_keys=md.shared_split_keys, split_tokens=md.shared_split_tokens,
-                out=self._out_buffer(layer_idx, b), workspace=self._shared_ws,
+                out=self._out_buffer(layer_idx, b), workspace=md.shared_ws,
                 device_error=self.device_error, seq_order=md.seq_order,
             ).view(b, 1, hq, d)
         elif tq == 1:
@@ -823,7 +829,7 @@ class PagedCudaBackend(AttentionBackend):
             out = ops.paged_prefill(
                 query.reshape(b * tq, hq, d), k_pool, v_pool, md.block_tables, md.q_starts,
                 md.q_lens, md.ctx_before, tq, self.scale, device_error=self.device_error,
-                split_keys=split, workspace=self._prefill_ws if split else None,
+                split_keys=split, workspace=md.prefill_ws,
                 max_keys=md.key_len,
             ).view(b, tq, hq, d)
         if self.debug_invariants:
@@ -861,14 +867,14 @@ class PagedCudaBackend(AttentionBackend):
                 self.scale, self.split_tokens, out=out.view(b, tq, hq, d)[:, tq - 1],
                 workspace=self._workspace, device_error=err, seq_list=md.decode_list)
         if md.decode_list is None or md.num_prefill_seqs:
-            k, v = self._scratch
+            k, v = md.read_pools
             w = md.read_tables.shape[1]
             ops.cache_read_quant(*cache, md.block_tables[:, :w], md.read_lens, k, v,
                                  md.read_tables, err)
             split = md.prefill_split_keys
             out = ops.paged_prefill(flat, k, v, md.read_tables, md.q_starts, q_lens,
                                     md.ctx_before, tq, self.scale, out=out, device_error=err,
-                                    split_keys=split, workspace=self._prefill_ws if split else None,
+                                    split_keys=split, workspace=md.prefill_ws,
                                     max_keys=md.key_len)
         return out.view(b, tq, hq, d)
 

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import weakref
+
 import pytest
 import torch
 
@@ -61,6 +63,83 @@ def test_an_8_bit_reservation_is_reported(code):
     assert be.block_usage()["held_bytes"] == 8 * 16 * 2 * 2 * 2 * row
     be.free()
     assert be.k_scale is None and be.memory_stats().allocated_bytes == 0
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_a_steps_scratch_lives_as_long_as_its_metadata(code):
+    """A captured graph holds the addresses that its step was planned with: a later, larger step
+    takes a pool of its own."""
+    be = PagedCudaBackend(MODEL, device="cpu", dtype=torch.bfloat16, kv_codes=code)
+    be.allocate(2, 64)
+    zeros = torch.zeros(2, dtype=torch.int32)
+    tables = torch.arange(4, dtype=torch.int32).view(2, 2)
+    base = backend_module.PagedMetadata(
+        query_len=2, context_len=0, key_len=32, num_seqs=2, block_tables=tables, slot_mapping=zeros.long(),
+        positions=zeros.long(), ctx_lens=zeros, ctx_before=zeros, q_lens=zeros, q_starts=zeros, live_tokens=zeros)
+    first = be._plan_read(base, tables, zeros, 4)
+    held = [weakref.ref(x) for x in be._scratch]
+    second = be._plan_read(base, tables, zeros, 400)
+    assert be._scratch[0].shape[0] == 400 and all(r() is not None and r().shape[0] == 4 for r in held)
+    assert first.read_tables is not None and second.read_tables is not None  # both still in use
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["read back", "shared prefix", "split prefill"])
+def test_a_captured_step_survives_a_larger_one(kind, monkeypatch):
+    """forward() captured with one step's metadata, replayed after a step that needed more
+    scratch or workspace: the same outputs, and no write to memory that others now hold."""
+    monkeypatch.setattr(backend_module, "SHARED_MIN_VALUES", 1)
+    be = PagedCudaBackend(MODEL, device=DEV, dtype=torch.bfloat16, num_blocks=1400, split_tokens=32,
+                          kv_codes=torch.int8 if kind == "read back" else None,
+                          share_prefixes=kind == "shared prefix")
+    be.allocate(24, 8192)
+    mgr = be.make_block_manager(enable_prefix_caching=kind == "shared prefix")
+    if kind != "read back":
+        be.k_cache.normal_(0.0, 0.5)
+        be.v_cache.normal_(0.0, 0.5)
+    rng = torch.Generator().manual_seed(5)
+    new_id = iter(range(100))
+
+    def plan(rows, prompt, prefix):
+        """A prefill of `prompt` new tokens a row, or (prefix > 0) a decode behind a common prompt."""
+        common = torch.randint(0, 50000, (prefix,), generator=rng).tolist()
+        ids = [next(new_id) for _ in range(rows)]
+        for i in ids:
+            own = torch.randint(0, 50000, (prompt,), generator=rng).tolist()
+            mgr.allocate(i, prefix + prompt, common + own)
+            if prefix:
+                mgr.schedule([i])
+                mgr.append_slots(i, 1, [7])
+        return mgr.schedule(ids)
+
+    def size():
+        held = {"read back": be._scratch and be._scratch[0], "shared prefix": be._shared_ws,
+                "split prefill": be._prefill_ws}[kind]
+        return 0 if held is None else held.numel() * held.element_size()
+
+    small = {"read back": (2, 40, 0), "shared prefix": (3, 9, 64), "split prefill": (1, 2000, 0)}[kind]
+    large = {"read back": (2, 900, 0), "shared prefix": (20, 9, 1024), "split prefill": (1, 6000, 0)}[kind]
+    p = plan(*small)
+    md = be.begin_plan(p)
+    first = size()
+    assert first > 0 and (kind != "shared prefix" or md.group_starts is not None)
+    b, tq = len(p.seq_ids), p.query_len
+    q, k, v = ((torch.randn((b, tq, h, 128), generator=rng) * 0.5).to(torch.bfloat16).to(DEV) for h in (8, 2, 2))
+    want = be.forward(0, q, k, v, md).clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = be.forward(0, q, k, v, md)
+    be.begin_plan(plan(*large))
+    assert size() > first
+    torch.cuda.synchronize()
+    junk = [torch.full((first,), 77, dtype=torch.uint8, device=DEV) for _ in range(64)]
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    assert all((j == 77).all() for j in junk)
+    assert int(be.device_error) == 0
 
 
 class _History:
