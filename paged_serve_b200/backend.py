@@ -542,7 +542,9 @@ class PagedCudaBackend(AttentionBackend):
             query_len=tq, context_len=max(plan.ctx_before), key_len=max(lens), num_seqs=b,
             block_tables=tables, slot_mapping=slots, positions=positions,
             ctx_lens=ctx_lens, ctx_before=ctx_before, q_lens=q_lens,
-            q_starts=q_starts, live_tokens=live, seq_order=self._decode_order(ctx_lens, tq),
+            q_starts=q_starts, live_tokens=live,
+            # under shared prefixes _plan_shared orders by the keys behind them
+            seq_order=self._decode_order(ctx_lens, tq) if groups is None else None,
             decode_list=decode_list, prefill_q_lens=prefill_q_lens,
             num_prefill_seqs=sum(1 for n in plan.q_lens if n > 1),
         )

@@ -321,6 +321,33 @@ def test_continuous_batching_with_shared_prefixes(split, monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("share", [True, False])
+def test_a_step_sorts_its_sequences_once(share, monkeypatch):
+    """By their own keys where prefixes are shared, else by their lengths."""
+    monkeypatch.setattr(backend_module, "SHARED_MIN_VALUES", 1)
+    be = PagedCudaBackend(MODEL, device=DEV, dtype=torch.bfloat16, num_blocks=96, share_prefixes=share)
+    be.allocate(4, 512)
+    mgr = be.make_block_manager(enable_prefix_caching=True)
+    common = list(range(64))
+    for i, own in enumerate((40, 5, 90)):
+        mgr.allocate(i, 64 + own, common + [100 + i] * own)
+        mgr.schedule([i])
+        mgr.append_slots(i, 1, [7])
+    sorted_by = []
+    order = backend_module.ops.decode_order
+
+    def counted(lens, **kw):
+        sorted_by.append(lens.tolist())
+        return order(lens, **kw)
+
+    monkeypatch.setattr(backend_module.ops, "decode_order", counted)
+    md = be.begin_plan(mgr.schedule([0, 1, 2]))
+    assert (md.group_starts is not None) == share
+    assert sorted_by == ([[41, 6, 91]] if share else [[105, 70, 155]])
+    assert md.seq_order.tolist() == [2, 0, 1]
+
+
+@pytest.mark.gpu
 def test_small_savings_keep_the_plain_decode():
     be = PagedCudaBackend(MODEL, device=DEV, dtype=torch.bfloat16, num_blocks=96, split_tokens=32,
                           share_prefixes=True)
