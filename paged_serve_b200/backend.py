@@ -570,7 +570,8 @@ class PagedCudaBackend(AttentionBackend):
     def _min_shared_keys(self) -> int:
         """Keys a shared-prefix decode must save a layer to be worth its prefix pass."""
         m = self.model
-        return SHARED_MIN_VALUES // (m.num_kv_heads * m.head_dim)
+        values = SHARED_MIN_VALUES * (m.num_layers + 11) // m.num_layers
+        return values // (m.num_kv_heads * m.head_dim)
 
     def _plan_shared(self, md: PagedMetadata, groups, lens: list[int], starts: torch.Tensor,
                      shared: torch.Tensor) -> PagedMetadata:
@@ -948,12 +949,16 @@ class PagedCudaBackend(AttentionBackend):
 
 
 # K (or V) values a shared-prefix decode must save a layer before it replaces the plain decode:
-# saved keys x KV heads x head dim. Its prefix pass costs about 7 to 15 us of launches and
-# lookups, what reading these takes. One group, a layer's append and decode, plain against
-# shared: Hq 32, Hkv 8, D 128, 16 rows over 1024 keys (15 M values) 21.5 / 24.6 us, 4 over
-# 16384 (48 M) 41.0 / 37.4, 64 over 4096 (252 M) 108.6 / 39.9; Hq 14, Hkv 2, D 64, 64 over
-# 1024 (8 M) 15.4 / 20.5, 64 over 4096 (31 M) 25.1 / 24.1.
-SHARED_MIN_VALUES = 1 << 25
+# saved keys x KV heads x head dim, this many times 1 + 11 / layers. A layer takes two calls for
+# one (10 us of host time and 7 to 15 us of launches and lookups on the device), what reading the
+# first part takes; the step finds its groups once and plans them (0.05 to 0.25 ms), which few
+# layers spread thinly. Whole eager steps, begin_plan included, plain / shared: 32 layers, Hq 32,
+# Hkv 8, D 128: 16 rows over 4096 keys (60 Mi values) 1.35 / 1.41 ms, 64 over 1024 (63 Mi)
+# 1.46 / 1.47, 64 over 2048 (126 Mi) 2.20 / 1.48; 80 layers of Hq 64: 64 over 512 (31.5 Mi)
+# 2.68 / 3.23, 64 over 1024 (63 Mi) 3.57 / 3.23; 24 layers of Hq 14, Hkv 2, D 64: 256 over 1024
+# (32 Mi) 1.02 / 1.41, 256 over 4096 (127 Mi) 2.11 / 1.58; 4 of them: 256 over 4096 0.67 / 0.80,
+# 256 over 8192 (255 Mi) 1.00 / 0.99.
+SHARED_MIN_VALUES = 3 << 24
 
 
 _ID_BYTES = array("i").itemsize
@@ -985,8 +990,10 @@ def shared_groups(tables, lens, block_size: int, min_saved: int):
     grows while that saves more keys ((rows - 1) x shared tokens), and only whole blocks
     behind which every row has a token of its own are shared.
     """
-    raw = [(t if isinstance(t, array) else array("i", t)).tobytes() for t in tables]
     blocks = [min(len(t), max(x - 1, 0) // block_size) for t, x in zip(tables, lens, strict=True)]
+    if sum(blocks) * block_size < min_saved:
+        return None  # not even if all of them were shared
+    raw = [(t if isinstance(t, array) else array("i", t)).tobytes() for t in tables]
     first, pre = [0], []
     saved = 0
     n = len(raw)

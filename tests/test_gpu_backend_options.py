@@ -196,6 +196,20 @@ def test_a_captured_step_survives_a_larger_one(kind, monkeypatch):
     assert int(be.device_error) == 0
 
 
+@pytest.mark.parametrize("layers,heads,rows,prefix,worth", [
+    (32, (32, 8, 128), 16, 4096, False), (32, (32, 8, 128), 64, 2048, True), (80, (64, 8, 128), 64, 512, False),
+    (80, (64, 8, 128), 64, 1024, True), (24, (14, 2, 64), 256, 1024, False), (24, (14, 2, 64), 256, 4096, True),
+    (4, (14, 2, 64), 256, 4096, False)])
+def test_groups_are_taken_where_whole_steps_get_shorter(layers, heads, rows, prefix, worth):
+    """Each measured as whole steps of both kinds (the figures beside SHARED_MIN_VALUES)."""
+    model = ModelConfig(name="m", num_layers=layers, num_q_heads=heads[0], num_kv_heads=heads[1], head_dim=heads[2])
+    be = PagedCudaBackend(model, device="cpu", dtype=torch.bfloat16, share_prefixes=True)
+    common = list(range(prefix // BS))
+    tables = [array("i", common + [5000 + i]) for i in range(rows)]
+    got = shared_groups(tables, [prefix + 5] * rows, BS, be._min_shared_keys())
+    assert got == (([0, rows], [prefix] * rows) if worth else None)
+
+
 class _History:
     """Token ids per sequence and the K/V a model would produce for them, prefix by prefix."""
 
