@@ -229,6 +229,25 @@ def test_decode_vs_float64(code, dtype, hq, hkv, d, bs, split):
 
 
 @pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,d,bs", [(32, 2, 128, 16), (27, 3, 128, 8), (20, 2, 128, 32), (30, 3, 64, 8),
+                                         (12, 1, 64, 16)])
+@pytest.mark.parametrize("split", [0, 64])
+def test_decode_with_more_than_eight_heads_vs_float64(code, dtype, hq, hkv, d, bs, split):
+    """Both head tiles, full and part full, at every block size."""
+    nb = sum((n + bs - 1) // bs for n in LENS) + 7
+    cache = _random_cache(nb, hkv, bs, d, code, seed=hq + bs)
+    tables = random_tables(LENS, bs, nb, seed=31, width=1024 // bs + 1)
+    _spoil_tails(cache, tables, LENS)
+    q = torch.randn((len(LENS), hq, d), device=DEV, generator=_gen(32)).to(dtype)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = _decode(q, cache, tables.to(DEV), torch.tensor(LENS, dtype=torch.int32, device=DEV), split,
+                  device_error=err)
+    assert int(err) == 0
+    _check_decode(out, q, cache, tables, LENS, f"{code} {dtype} {hq}/{hkv} d{d} bs{bs} split{split}")
+
+
+@pytest.mark.parametrize("code", CODES)
 def test_decode_with_wide_ranges(code):
     """Loud tokens among quiet ones (V scales over six decades, in rising and falling
     order), large scores and queries of large and small size."""

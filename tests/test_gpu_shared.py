@@ -9,7 +9,7 @@ import torch
 
 from paged_serve_b200 import _lib, ops
 from tests.gpu_util import random_pool
-from tests.quant_util import assert_within, attend, quantise, sequence
+from tests.quant_util import assert_within, attend, dequantise, quantise, sequence
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -311,3 +311,28 @@ def test_over_a_read_back_cache(code):
         # the read-back values are off by bf16's half step, 2^-8 of v and, through the
         # scores (|s| <= 2^4 in all), at most 2^-8 * 2^4 of a probability
         assert_within(direct[b], ref, weight * (2.0**-4 + 2.0**-8) / 2.0**-11, f"row {b}")
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("split", [0, 32])
+def test_a_read_back_prefix_and_the_codes_agree(code, split):
+    """The decode over the codes against float64 over what the codes stand for, at its own
+    roundings, on the tables of a shared prompt; and the shared path over the values read back
+    against float64 over those."""
+    pre, starts, lens, tables, nb = _case([(9, 320)], [(11 * i) % 50 + 1 for i in range(9)], 16, seed=2)
+    g = torch.Generator(device=DEV).manual_seed(13)
+    kp, ks = quantise(torch.randn((nb, 8, 16, 128), device=DEV, generator=g), code)
+    vp, vs = quantise(torch.randn((nb, 8, 16, 128), device=DEV, generator=g), code)
+    q = torch.randn((9, 32, 128), device=DEV, generator=g).to(torch.bfloat16)
+    dt, ctx = tables.to(DEV), _i32(lens)
+    ws = torch.empty(max(256, ops.decode_workspace_bytes(9, 32, 128, 16, dt.shape[1], split)), dtype=torch.uint8,
+                     device=DEV)
+    direct = ops.paged_decode_quant(q, kp, vp, ks, vs, dt, ctx, 128**-0.5, split, workspace=ws)
+    pools = [torch.full((nb, 8, 16, 128), NAN, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    ops.cache_read_quant(kp, vp, ks, vs, dt, ctx, *pools, dt)
+    out = _shared(q, pools, tables, lens, pre, starts, 128, split)
+    for b, n in enumerate(lens):
+        k, v = (dequantise(sequence(c, dt[b], n), sequence(s, dt[b], n)) for c, s in ((kp, ks), (vp, vs)))
+        ref, weight = attend(q[b], k, v, 128**-0.5)
+        assert_within(direct[b], ref, weight, f"codes, row {b}")
+    _check(out, q, pools, tables, lens, "read back")
