@@ -63,7 +63,8 @@ int encode_tmap(CUtensorMap* map, CUtensorMapDataType type, void* base, int rank
     estride[i] = 1;
     if (i > 0) gstride[i - 1] = strides_bytes[i - 1];
   }
-  CUresult r = g_encode(map, type, rank, base, gdim, gstride, bdim, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+  CUresult r = g_encode(map, type, rank, base, gdim, gstride, bdim, estride,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return fail(PS_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));

@@ -570,24 +570,10 @@ int launch_decode(const DecodeParams& p, const CUtensorMap& km, const CUtensorMa
   static size_t configured[64] = {};
   int st = reserve_smem(kern, smem, configured);
   if (st != PS_OK) return st;
-  static int occ_dev[64], occ_blocks[64];
-  static size_t occ_smem[64] = {};
-  int dev = 0, sms = 148, per_sm = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int slot = (dev >= 0 && dev < 64) ? dev : 0;
-  std::unique_lock<std::mutex> lock(g_launch_mu);
-  if (occ_smem[slot] == smem && occ_dev[slot] == dev) {
-    per_sm = occ_blocks[slot];
-  } else {
-    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kNW * 32, smem);
-    if (e != cudaSuccess || per_sm <= 0)
-      return fail(PS_ERR_CUDA, "ps_paged_decode: occupancy query failed: %s", cudaGetErrorString(e));
-    occ_smem[slot] = smem;
-    occ_dev[slot] = dev;
-    occ_blocks[slot] = per_sm;
-  }
-  lock.unlock();
+  static Resident cache[64];
+  Resident res;
+  st = resident_ctas(kern, "ps_paged_decode", kNW * 32, smem, cache, &res);
+  if (st != PS_OK) return st;
   cudaError_t e = cudaSuccess;
   if (!p.planned) {
     e = launch_pdl(decode_plan_kernel<kShared>, dim3(1), dim3(1024), 0, s, p);
@@ -598,7 +584,7 @@ int launch_decode(const DecodeParams& p, const CUtensorMap& km, const CUtensorMa
     st = launch_shared_prefix(*prefix, s);
     if (st != PS_OK) return st;
   }
-  e = launch_pdl(kern, dim3(per_sm * sms), dim3(kNW * 32), smem, s, p, km, vm);
+  e = launch_pdl(kern, dim3(res.per_sm * res.sms), dim3(kNW * 32), smem, s, p, km, vm);
   if (e != cudaSuccess)
     return fail(PS_ERR_CUDA, "ps_paged_decode: launch failed: %s", cudaGetErrorString(e));
   const int warps = p.num_launch * p.num_q_heads;
@@ -871,16 +857,6 @@ extern "C" int ps_paged_decode_plan(const int32_t* ctx_lens, int num_seqs,
   if (num_seqs == 0 || max_splits <= 1) return PS_OK;  // nothing is split: no plan
   if (max_splits > 65535) return fail(PS_ERR_INVALID, "%s: too many partitions", fn);
   if (!ctx_lens) return fail(PS_ERR_INVALID, "%s: null ctx_lens", fn);
-  const int64_t need = ps_paged_decode_workspace_bytes(num_seqs, num_q_heads, head_dim, block_size,
-                                                       max_blocks_per_seq, split_tokens);
-  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
-    return fail(PS_ERR_INVALID, "%s: needs a 256-byte aligned workspace of %lld bytes", fn,
-                (long long)need);
-  const int64_t rows_ws = static_cast<int64_t>(num_seqs) * max_splits * num_q_heads;
-  const int64_t o_bytes = ((rows_ws * head_dim * 4) + 255) / 256 * 256;
-  const int64_t lse_bytes = ((rows_ws * 4) + 255) / 256 * 256;
-  const int64_t item_bytes = ((static_cast<int64_t>(num_seqs) * max_splits * 4) + 255) / 256 * 256;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
   DecodeParams p{};
   p.ctx_lens = ctx_lens;
   p.num_seqs = num_seqs;
@@ -890,9 +866,10 @@ extern "C" int ps_paged_decode_plan(const int32_t* ctx_lens, int num_seqs,
   p.part_tokens = part;
   p.max_splits = max_splits;
   p.seq_order = seq_order;
-  p.items = reinterpret_cast<int32_t*>(ws + o_bytes + lse_bytes);
-  p.item_count = reinterpret_cast<int32_t*>(ws + o_bytes + lse_bytes + item_bytes);
-  p.item_next = p.item_count + 1;
+  const int st = set_split_workspace(fn, &p, num_seqs, num_q_heads, head_dim, block_size,
+                                     max_blocks_per_seq, split_tokens, max_splits, workspace,
+                                     workspace_bytes);
+  if (st != PS_OK) return st;
   const cudaError_t e =
       launch_pdl(decode_plan_kernel<false>, dim3(1), dim3(1024), 0, as_stream(stream), p);
   if (e != cudaSuccess) return fail(PS_ERR_CUDA, "%s: launch failed: %s", fn, cudaGetErrorString(e));

@@ -503,7 +503,6 @@ __device__ __forceinline__ bool softmax_tile(const PrefillParams& p, uint64_t* b
   return true;
 }
 
-// BS = tokens per KV block (8, 16 or 32): a 128-key tile is 128/BS block boxes.
 // Shared-prefix pass: sets an error bit unless the groups are in order and every row with
 // a prefix is in one whose rows all have its length (a row outside would merge partials that
 // nothing has written). As the groups leave no gaps, that is: a row whose length
@@ -533,6 +532,7 @@ __device__ __forceinline__ void check_groups(const PrefillParams& p, int lane) {
   if (bad) set_device_error(p.err, PS_DEVERR_LENGTH);
 }
 
+// BS = tokens per KV block (8, 16 or 32): a 128-key tile is 128/BS block boxes.
 template <typename T, int D, int BS, bool kSplit, bool kShared>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap qmap,

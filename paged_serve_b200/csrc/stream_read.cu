@@ -54,6 +54,15 @@ constexpr size_t kBulkSmem = kBulkWarps * kBulkStages * (kBulkChunk + 8) + 128;
 
 __device__ __forceinline__ int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
 
+__device__ __forceinline__ void bulk_g2s(void* dst, const void* src, uint32_t bytes,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // Every wait is bounded: a timeout sets PS_DEVERR_TIMEOUT, and the warp waits
 // (bounded again) for its copies still in flight before the CTA's shared
 // memory goes away.
