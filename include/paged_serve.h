@@ -598,7 +598,8 @@ PS_API int ps_cache_read_quant(const void* k_pool, const void* v_pool, const flo
  * softmax and accumulation are float32; probabilities times V scales are rounded to fp16
  * for the second product (a probability below 2^-126 of the largest counts as 0). As in
  * ps_paged_decode the sum of p |v| before the division, p = 1 at the largest score, must stay
- * in float32's range.
+ * in float32's range. Queries are held in fp16 relative to the power of two at their head's
+ * largest element: 2^-25 of that is the most an element loses.
  */
 PS_API int ps_paged_decode_quant(void* out, int64_t out_seq_stride, const void* query,
                                  int64_t query_seq_stride, const void* k_pool, const void* v_pool,

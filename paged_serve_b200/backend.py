@@ -168,11 +168,15 @@ class PagedCudaBackend(AttentionBackend):
             kv_codes: ``torch.float8_e4m3fn`` or ``torch.int8`` holds the cache in 8
                 bits with a float32 scale per (token, KV head) row; None in ``dtype``.
                 A prefilling sequence's tokens are read back into a 16-bit scratch
-                pool of its own length, shared by the layers.
+                pool shared by the layers, allocated by the step that first needs its
+                size (a step's prefilling sequences whole, context and new tokens), outside what
+                :meth:`allocate` reserves. A mixed step runs its decode, read-back and
+                prefill one after another (``overlap_mixed_steps`` has no effect).
             share_prefixes: a decode step planned by the block manager reads leading
                 blocks that neighbouring sequences of the plan share once for the
                 group, where that saves enough keys (:func:`shared_groups`); not with
-                ``kv_codes``. Schedule sequences of one prompt next to each other.
+                ``kv_codes``, nor in steps over static metadata (:meth:`load_decode_plan`,
+                decode graphs). Schedule sequences of one prompt next to each other.
         """
         if model.num_q_heads % model.num_kv_heads != 0:
             raise ValueError("num_q_heads must be divisible by num_kv_heads")

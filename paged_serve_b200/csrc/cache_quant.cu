@@ -136,8 +136,9 @@ __global__ void __launch_bounds__(256)
 
 // With RoPE on K: the CTAs of blockIdx.y 0 take the K rows, those of 1 the V rows. The
 // rotation's chain of loads (position, then its cos and sin) wants more warps than the
-// registers of both rows at once leave: 22.0 us against 24.1 in one thread (the sizes
-// above; without a rotation the split costs 1.5 us).
+// registers of both rows at once leave: 23.2 us against 24.6 in one thread (the sizes
+// above; without a rotation the split costs 1.5 us). Position, slot, cos and sin are fetched
+// and unpacked once per head: 70% of the issue slots, of which the rows' own work is a part.
 // K is rotated in fp32: the products of two 16-bit values are exact there, so
 // each rotated element is rounded once before it is quantised.
 template <typename T, int D, typename C>

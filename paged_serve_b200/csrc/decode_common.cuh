@@ -91,7 +91,7 @@ struct SharedRows {
 // Adds a prefix's partials to one column of four of a row: m, l, acc = running maximum,
 // sum and unnormalised output. Eight partials' loads are in flight at a time, also where
 // fewer are left: one after the other they were 9,300 of a CTA's 35,000 cycles at 256
-// sequences over 4 partials (112 us a call against 118).
+// sequences over 4 partials (112 us a call against 117).
 template <int D>
 __device__ __forceinline__ void merge_shared(const DecodeParams& p, const SharedRows& rows,
                                              int parts, int col4, float& m, float& l,

@@ -5,9 +5,11 @@
 //   s_n = scale * a_n * (q . k_n)     o = sum_n softmax(s)_n * b_n * v_n
 // so both scales stay outside the matrix products: a_n multiplies a score, b_n a
 // probability. The products run on fp16 warp MMAs: every e4m3 or int8 code is an
-// fp16 value, so only the probabilities are rounded (2^-12 relative); the
-// queries are first brought to [-2, 2) per head by a power of two (exact, up to
-// values below 2^-24 of the head's largest).
+// fp16 value, so the probabilities are rounded (2^-11 relative), and the queries
+// where a head's elements differ most: each head is first brought to [-2, 2) by a
+// power of two, and there fp16's step is 2^-24 from 2^-14 down. Elements below 2^-14 (bf16
+// queries, of fewer bits: 2^-17) of that range lose low bits, 2^-25 at most, and those
+// below 2^-25 all of them: per product what fp32 sums of the larger ones lose too.
 //
 // A probability times b_n must fit fp16 too, whatever the b_n are, and keep its
 // precision where the sum has its weight. So beside the running maximum m of the
@@ -35,9 +37,10 @@
 // of the MMA's k indices they stand for is free as long as Q is laid out alike.
 //
 // Bound by HBM, with half the bytes of the 16-bit cache to hide the same work behind:
-// 256 sequences U[512,4096], Hq 32, Hkv 8, D 128, e4m3, blocks of 16 take 191-209 us by
-// box for 1.293 GB (6,190-6,790 GB/s, 0.96-1.05 of the copy peak; the 16-bit cache takes
-// 347 us). A warp spends 1,200-1,500 cycles on a stage of 32 keys and about 800 on
+// 256 sequences U[512,4096], Hq 32, Hkv 8, D 128, e4m3, blocks of 16 take 190-209 us by
+// box for 1.293 GB (6,190-6,820 GB/s; the 16-bit cache takes 347 us). That is 0.96-1.05 of
+// a copy's rate, which pays for writes too; of a plain read of as many bytes
+// (ps_stream_read, 7,030-7,130 GB/s on the box of the 190 us) it is 0.96. A warp spends 1,200-1,500 cycles on a stage of 32 keys and about 800 on
 // issuing the next one; twelve warps per SM hide both. Measured and not kept: 2 to 16
 // warps of 1 to 4 stages and stages of 16 keys (193 to 324 us); a producer warp per CTA
 // feeding four others through a shared ring (870 cycles to issue a stage: 226 us with
@@ -625,6 +628,11 @@ int launch_quant(const QuantDecodeParams& qp, const CUtensorMap& km, const CUten
   return check_launch(fn);
 }
 
+// Nine heads and more take a second head tile (R 16): at head dim 128 its fragments and
+// accumulators bring the kernel from 123-168 registers to 168-226, which leaves two CTAs an SM
+// in place of three in all but a few forms. 256 sequences U[512,4096], Hkv 2, D 128, e4m3: 8 heads a KV head 59.1 us, 16 heads
+// 64.8 (int8 78.4, blocks of 8 75.1) for the same keys, whose bytes take 50.5; in partitions
+// of 512 keys 74.8 and 114.1.
 template <typename T, typename C, int D>
 int dispatch_geometry(const QuantDecodeParams& p, const CUtensorMap& km, const CUtensorMap& vm,
                       cudaStream_t s) {

@@ -41,6 +41,10 @@
 // the burst peak, bound by the per-tile chain and, with 16 key tiles a unit, by a unit's
 // start and end (about five key tiles' time). 8 rows of 8 heads over 32768 keys (134 MB):
 // 42 us in 16 pieces of paired tiles, 0.50 of the copy peak.
+// P is rounded to the pools' type for the second product (2^-8 of a probability in bf16, 2^-11
+// in fp16, one term) and the row sums add it unrounded, as in the prefill; the decode of the own
+// keys rounds alike and sums what it rounded. So the two parts of one softmax are
+// normalised apart by less than those roundings, which average out over a row's keys.
 //
 // All waits are bounded; a timeout sets PS_DEVERR_TIMEOUT and a shared abort
 // flag so every role leaves its loop, drains its in-flight copies / MMAs and

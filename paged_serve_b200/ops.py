@@ -66,8 +66,9 @@ def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
 
 
 def _stream(device: torch.device) -> int:
-    # The handle of torch.cuda.current_stream(device) without making a Stream object
-    # (3.8 us of host time a call).
+    # The handle of torch.cuda.current_stream(device) without making a Stream object (3.8 us
+    # of a call's 8 to 20 us on the host), by the function under that property; torch
+    # documents neither that one nor another way to the bare handle.
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
