@@ -40,9 +40,9 @@
 // 256 sequences U[512,4096], Hq 32, Hkv 8, D 128, e4m3, blocks of 16 take 190-209 us by
 // box for 1.293 GB (6,190-6,820 GB/s; the 16-bit cache takes 347 us). That is 0.96-1.05 of
 // a copy's rate, which pays for writes too; of a plain read of as many bytes
-// (ps_stream_read, 7,030-7,130 GB/s on the box of the 190 us) it is 0.96. A warp spends 1,200-1,500 cycles on a stage of 32 keys and about 800 on
-// issuing the next one; twelve warps per SM hide both. Measured and not kept: 2 to 16
-// warps of 1 to 4 stages and stages of 16 keys (193 to 324 us); a producer warp per CTA
+// (ps_stream_read, 7,030-7,130 GB/s on the box of the 190 us) it is 0.96. A warp spends
+// 1,200-1,500 cycles on a stage of 32 keys and about 800 on issuing the next one; twelve
+// warps per SM hide both. Measured and not kept: 2 to 16 warps of 1 to 4 stages and stages of 16 keys (193 to 324 us); a producer warp per CTA
 // feeding four others through a shared ring (870 cycles to issue a stage: 226 us with
 // TMA, 202 us with 16-byte asynchronous copies); persistent CTAs taking over pending
 // ones with the next unit's keys prefetched during the merge (no gain: the other CTAs of
@@ -630,9 +630,9 @@ int launch_quant(const QuantDecodeParams& qp, const CUtensorMap& km, const CUten
 
 // Nine heads and more take a second head tile (R 16): at head dim 128 its fragments and
 // accumulators bring the kernel from 123-168 registers to 168-226, which leaves two CTAs an SM
-// in place of three in all but a few forms. 256 sequences U[512,4096], Hkv 2, D 128, e4m3: 8 heads a KV head 59.1 us, 16 heads
-// 64.8 (int8 78.4, blocks of 8 75.1) for the same keys, whose bytes take 50.5; in partitions
-// of 512 keys 74.8 and 114.1.
+// in place of three in all but a few forms. 256 sequences U[512,4096], Hkv 2, D 128, e4m3:
+// 8 heads a KV head 58-59 us, 16 heads 64-65 (int8 78, blocks of 8 75) for the same keys,
+// whose bytes take 50.5; in partitions of 512 keys 74-75 and 114.
 template <typename T, typename C, int D>
 int dispatch_geometry(const QuantDecodeParams& p, const CUtensorMap& km, const CUtensorMap& vm,
                       cudaStream_t s) {
