@@ -93,6 +93,19 @@ def test_decode_refusals():
     assert _decode(split=16, ws=256, wsb=100) == _lib.PS_ERR_INVALID
 
 
+def test_plan_refusals():
+    def plan(b=4, mb=64, split=16, ws=256, wsb=1 << 62):
+        return _lib.load().ps_paged_decode_plan(16, b, None, 8, 128, 16, mb, split, ws, wsb, None)
+
+    assert plan(ws=None) == _lib.PS_ERR_INVALID and "workspace" in _msg()
+    assert plan(ws=16) == _lib.PS_ERR_INVALID
+    assert plan(wsb=100) == _lib.PS_ERR_INVALID and "workspace" in _msg()
+    assert plan(split=24) == _lib.PS_ERR_INVALID
+    # 65,535 sequences of 40,000 partitions: more units than 32 bits count
+    assert plan(b=65535, mb=40000) == _lib.PS_ERR_INVALID and "units" in _msg()
+    assert plan(mb=1) == _lib.PS_OK  # nothing is split
+
+
 def test_ops_refuse_host_tensors():
     kp = torch.zeros((2, 1, 16, 64), dtype=torch.int8)
     sc = torch.zeros((2, 1, 16))
